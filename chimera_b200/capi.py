@@ -56,12 +56,26 @@ class SearchParams(C.Structure):
                 ("table_log2_extra", C.c_int32)]
 
 
+class ChmHeads(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("heads", C.c_int32), ("batch_stride", C.c_int64),
+                ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class ChmKvCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("num_pages", C.c_int64), ("page_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("token_stride", C.c_int64), ("page_size", C.c_int32), ("heads", C.c_int32), ("dim", C.c_int32),
+                ("type", C.c_int32)]
+
+
 _lib_handle = None
 _rng_handle = None
 V = C.c_void_p
 I64 = C.c_int64
 I32 = C.c_int32
 SZ = C.c_size_t
+F32 = C.c_float
+F64 = C.c_double
 
 EXPORTS = {
     "chm_version": ([], C.c_char_p),
@@ -100,6 +114,12 @@ EXPORTS = {
     "chm_token_clusters": ([V, I64, V, I64, V, V], C.c_int),
     "chm_stage1_table_queries": ([V, I32, I32, I32, I32, V, SZ, V, V], C.c_int),
     "chm_build_cluster_order_workspace_bytes": ([I64, I64], SZ),
+    "chm_rotary_frequencies": ([I32, F64, I32, F64, F64, F64, F64, V], C.c_int),
+    "chm_rotary": ([V, V, I32, I32, I64, I64, I32, I32, V, I32, I64, I64, V, F32, I32, V], C.c_int),
+    "chm_cache_write": ([V, V, V, I32, I64, V, V], C.c_int),
+    "chm_cache_read": ([V, V, I64, V, V, I32, V], C.c_int),
+    "chm_paged_attention_workspace_bytes": ([V, I64, I32, I32], SZ),
+    "chm_paged_attention": ([V, V, V, I32, I64, V, I64, I32, V, V, F32, V, V, SZ, V], C.c_int),
     "chm_build_cluster_order": ([V, I64, I64, V, I64, V, V, V, V, V, V, V, V, V, V, SZ, V], C.c_int),
 }
 

@@ -346,6 +346,119 @@ chm_status chm_token_clusters(const int64_t* cluster_pos, int64_t n_clusters, co
 /* ||x||^2 of n rows of width 128 as a sequential fma chain. */
 chm_status chm_row_norms(const float* x, int64_t n, float* out, void* stream);
 
+/*
+ * Generation over cached keys and values: the reader that answers from the
+ * documents a search returns walks token vectors much as the search does, with
+ * a softmax in place of the maximum.  No reference counterpart.
+ *
+ * These calls take CHM_FP32 / CHM_FP16 / CHM_BF16 vectors in any layout whose
+ * last axis is contiguous.  Null pointers, sizes below zero, unknown types and
+ * layouts a call does not take return CHM_ERR_INVALID (the reason in
+ * chm_last_error) and launch nothing; a batch of nothing returns CHM_OK.
+ */
+typedef enum { CHM_FP32 = 0, CHM_FP16 = 1, CHM_BF16 = 2, CHM_INT8 = 3, CHM_E4M3 = 4 } chm_type;
+
+/* Vectors [batch, tokens, heads, dim]; strides in elements, 1 along dim. */
+typedef struct {
+    void* data;
+    int32_t heads;
+    int64_t batch_stride, token_stride, head_stride;
+} chm_heads;
+
+/* Rotation frequencies (radians per position) of rot_dim / 2 pairs:
+ * base^(-2i / rot_dim), scaled for contexts longer than `original_len` by
+ * `factor` >= 1.  CHM_ROTARY_PLAIN: unscaled.  CHM_ROTARY_LINEAR: divided by
+ * the factor.  CHM_ROTARY_BASE: base * factor^(rot_dim / (rot_dim - 2)), so
+ * that the slowest pair is slowed by the factor and the fastest not at all.
+ * CHM_ROTARY_PARTS: a pair that turns r times over original_len keeps the
+ * share clamp((r - slow) / (fast - slow), 0, 1) of its frequency and takes the
+ * rest from the linear form.  Host function; freqs [rot_dim / 2] is host
+ * memory.  Takes 0 < slow < fast, base > 1. */
+typedef enum { CHM_ROTARY_PLAIN = 0, CHM_ROTARY_LINEAR = 1, CHM_ROTARY_BASE = 2, CHM_ROTARY_PARTS = 3 } chm_rotary_kind;
+chm_status chm_rotary_frequencies(int32_t rot_dim, double base, int32_t kind, double factor, double original_len,
+                                  double slow, double fast, double* freqs);
+
+/* Rotary positions: the first rot_dim of dim elements of every vector are
+ * rotated in pairs by angle positions[b, t] * freqs[i],
+ *   y0 = scale * (x0 cos a - x1 sin a),  y1 = scale * (x0 sin a + x1 cos a),
+ * the others are passed on.  Pair i is (i, i + rot_dim / 2), or (2i, 2i + 1)
+ * with CHM_ROTARY_INTERLEAVED.  CHM_ROTARY_INVERSE turns by -a: the gradient
+ * of the rotation (scale included).  `n` of 1 or 2 sets of heads (queries, and
+ * keys beside them) in one launch; out[i] has in[i]'s shape and may be in[i]
+ * itself (in place), but not overlap it in any other way.
+ * rot_dim is even, at most dim <= 4096.  positions: int64 or int32
+ * (position_bytes 8 or 4), strides in elements (batch stride 0: shared).
+ * Angles are reduced in 64 bits: their error stays below 1e-6 up to position
+ * 2^31. */
+#define CHM_ROTARY_INTERLEAVED 1
+#define CHM_ROTARY_INVERSE 2
+chm_status chm_rotary(const chm_heads* in, const chm_heads* out, int32_t n, int32_t type, int64_t batch,
+                      int64_t tokens, int32_t dim, int32_t rot_dim, const void* positions, int32_t position_bytes,
+                      int64_t position_batch_stride, int64_t position_token_stride, const double* freqs,
+                      float scale, int32_t flags, void* stream);
+
+/* A paged key-value cache: pages of page_size tokens of `heads` key and value
+ * vectors of `dim` elements.  Token s of the cache (its slot) sits in page
+ * s / page_size at s % page_size.  Element (page, head, token, d) of k and of v is
+ * at page * page_stride + head * head_stride + token * token_stride + d.
+ * type CHM_FP16 or CHM_BF16 holds the values, CHM_INT8 and CHM_E4M3 codes
+ * with one scale per vector: value = code * scale.  dim is a multiple of 16,
+ * at most 256; the strides are multiples of 16 bytes, k and v 16-byte aligned. */
+typedef struct {
+    void* k;
+    void* v;
+    float* k_scale; /* [num_pages, heads, page_size], contiguous; NULL for 16-bit types */
+    float* v_scale;
+    int64_t num_pages;
+    int64_t page_stride, head_stride, token_stride; /* elements */
+    int32_t page_size, heads, dim, type;
+} chm_kv_cache;
+
+/* Write tokens' key and value vectors (k, v: [tokens, heads, dim]; batch_stride
+ * unused) to the slots [tokens] (int64).  A slot below 0 or past the last page
+ * is skipped: padding.  A slot may stand once in a call (which of two tokens
+ * it would hold, or a mixture, is undefined).
+ * 8-bit types: scale = max |x| / 127 (int8) or / 448 (e4m3), rounded to fp32
+ * (down, where the top code would otherwise read back as an infinity);
+ * code = x / scale rounded to nearest, ties to even, as in exact arithmetic.
+ * A vector whose largest value is below 2^-96 is held as zeros; one with an
+ * infinity or a NaN gets a NaN scale, and every value of it reads back as NaN.
+ * 16-bit types: x rounded to the type. */
+chm_status chm_cache_write(const chm_kv_cache* cache, const chm_heads* k, const chm_heads* v, int32_t type,
+                           int64_t tokens, const int64_t* slots, void* stream);
+
+/* Read slots back: k, v [tokens, heads, dim] of `type`, code * scale in fp32
+ * rounded to the type.  A slot below 0 or past the last page reads as zeros.
+ * (e4m3: the NaN codes 0x7f and 0xff, which chm_cache_write never writes, count
+ * as +-480, here and in chm_paged_attention.) */
+chm_status chm_cache_read(const chm_kv_cache* cache, const int64_t* slots, int64_t tokens, const chm_heads* k,
+                          const chm_heads* v, int32_t type, void* stream);
+
+/* Attention of one new token per sequence over the cached ones:
+ *   out[b, h] = sum_j softmax_j(scale * <q[b, h], key_j>) value_j,
+ *   lse[b, h] = log sum_j exp(scale * <q[b, h], key_j>),  starts[b] <= j < lens[b],
+ * with token j of sequence b in page tables[b, j / page_size] and query heads
+ * h sharing key head h / (q_heads / cache->heads).
+ * q and out: [batch, q_heads, dim] of `type` (token_stride unused): fp16 or
+ * bf16, the cache's own type for 16-bit caches.  tables: int32
+ * [batch, table_width], rows table_stride apart; lens: int32 [batch]; starts:
+ * int32 [batch] or NULL for zeros (a window: lens - window; below 0 counts as
+ * 0); lse: fp32 [batch, q_heads] contiguous, or NULL.
+ * A row with nothing to attend to (lens <= starts), or whose scores are all
+ * -infinity, gets zeros and lse = -infinity.  Pages and parts of pages outside
+ * the range are not read.  A page id outside the cache that the range needs,
+ * or a length past the table's end, makes the sequence's rows and lse NaN.
+ * Softmax statistics and sums are fp32; probabilities enter the value product
+ * as two 16-bit terms (high and remainder).  Results do not depend on timing.
+ * table_width * page_size is at most 2^30, batch 65,535.  Calls on one
+ * workspace must not overlap. */
+size_t chm_paged_attention_workspace_bytes(const chm_kv_cache* cache, int64_t batch, int32_t q_heads,
+                                           int32_t table_width);
+chm_status chm_paged_attention(const chm_kv_cache* cache, const chm_heads* q, const chm_heads* out, int32_t type,
+                               int64_t batch, const int32_t* tables, int64_t table_stride, int32_t table_width,
+                               const int32_t* lens, const int32_t* starts, float scale, float* lse, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
