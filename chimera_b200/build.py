@@ -7,6 +7,8 @@
 * ``lib/libchimera_core.so`` -- the drop-in C++ ``Chimera::chimera_index``
   (include/chimera/chimera_index.cuh) over the C ABI.
 * ``chimera*.so`` (this directory) -- the pybind11 module ``chimera``.
+* ``_generation*.so`` (this directory) -- the generation operators over torch
+  tensors (chimera_b200/attention.py).
 * ``bin/gpu_build``, ``bin/gpu_search`` -- the drop-in CLI tools.
 
 Run ``python -m chimera_b200.build`` (or ``__graft_entry__.build()``).
@@ -132,6 +134,24 @@ def build_host(verbose=False):
     return core
 
 
+def build_generation():
+    """The operators of chimera_b200/attention.py over torch tensors."""
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    ext = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
+    mod = os.path.join(HERE, "_generation" + ext)
+    src = os.path.join(CSRC, "python", "generation.cpp")
+    if _stale(mod, [src, os.path.join(INCLUDE, "chimera_b200.h")]):
+        tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
+        inc = ["-isystem" + d for d in include_paths()] + ["-I" + INCLUDE, "-I" + os.path.join(CUDA_HOME, "include"),
+                                                          "-I" + sysconfig.get_paths()["include"]]
+        _run([_cxx(), "-std=c++17", "-O2", "-fPIC", "-shared", "-o", mod, src,
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + inc +
+             ["-L" + LIB, "-lchimera_b200", "-L" + tlib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+              "-Wl,-rpath,$ORIGIN/lib"])
+    return mod
+
+
 def build_hostrng():
     os.makedirs(LIB, exist_ok=True)
     so = os.path.join(LIB, "libchimera_hostrng.so")
@@ -143,6 +163,7 @@ def build_hostrng():
 
 def build(verbose=False, host=True):
     build_cuda(verbose)
+    build_generation()
     build_hostrng()
     if host:
         build_host(verbose)
