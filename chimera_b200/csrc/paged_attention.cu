@@ -11,6 +11,7 @@
 //   S^T [tokens x heads] = K [tokens x dim] Q^T,   O^T [dim x heads] += V^T P^T.
 // Both contractions may take their index in any order, so a thread's 16-byte
 // loads are its operand registers as they come: no shared memory, no barrier.
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 
@@ -23,6 +24,9 @@ constexpr int kAttThreads = kAttWarps * 32;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
+struct Plan;
+struct Boundary;
+
 struct AttArgs {
     chm_kv_cache c;
     const void* q;
@@ -33,7 +37,12 @@ struct AttArgs {
     int32_t blocks;                 // blocks of 8 * NT query heads per key head
     const int32_t* tables;
     int64_t table_stride;
-    int32_t capacity;  // table_width * page_size
+    int32_t capacity;     // table_width * page_size
+    int32_t unit_tokens;  // tokens per unit of work
+    FastDiv by_unit;
+    Plan* plan;
+    Boundary* boundaries;
+    float* parts;
     const int32_t* lens;
     const int32_t* starts;
     float scale_log2;
@@ -118,326 +127,603 @@ __device__ __forceinline__ uint32_t codes_to_bf16(uint32_t y) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// What one lane knows of one token of a step: where it is, and its scales.
-struct TokenInfo {
-    int64_t at;  // element offset of its vector, -1: none
-    float ks, vs;
+// ---- how the work is split ------------------------------------------------------
+//
+// A segment is one sequence's tokens for one block of query heads that share a
+// key head.  It is cut into tiles (a step of all warps), and the tiles of all
+// segments, in the order (sequence, block, tile), are dealt out evenly: with
+// `per` = ceil(units / blocks), block c takes units [c * per, (c + 1) * per).
+// So the lengths, which only the device knows, do not matter to the balance, a
+// long sequence spreads over the device and short ones stay whole.  A segment
+// that crosses a block boundary leaves a part (unnormalised output, maximum,
+// sum) per block in the workspace, and attention_join_kernel adds them in order.
+struct Plan {
+    int per;    // units per block
+    int total;  // units
+};
+struct Boundary {  // the first segment of a block
+    int seq, seg;
+    int first, units;  // its first unit, its units
 };
 
-// One sequence's attended range and the walk over its table.
-struct Sequence {
-    int first, end;  // positions
-    const int32_t* table;
+struct Range {
+    int first, end;  // positions attended to
+    int units;
+    bool bad;  // the length does not fit the table
 };
 
-template <int KIND>
-__device__ __forceinline__ TokenInfo token_info(const AttArgs& a, const Sequence& s, int pos, int head, bool& bad) {
-    TokenInfo r{-1, 0.0f, 0.0f};
-    if (pos < s.end) {
-        const uint32_t pi = a.by_page.div((uint32_t)pos);
-        const uint32_t within = (uint32_t)pos - pi * (uint32_t)a.c.page_size;
-        const int64_t page = s.table[pi];
-        if (page < 0 || page >= a.c.num_pages) {
-            bad = true;
-        } else {
-            r.at = page * a.c.page_stride + (int64_t)head * a.c.head_stride + (int64_t)within * a.c.token_stride;
-            if (KIND == CHM_INT8 || KIND == CHM_E4M3) {
-                const int64_t i = (page * a.c.heads + head) * a.c.page_size + within;
-                r.ks = a.c.k_scale[i];
-                r.vs = a.c.v_scale[i];
-            }
-        }
-    }
+__device__ __forceinline__ Range sequence_range(const AttArgs& a, int b) {
+    Range r;
+    r.first = a.starts ? min(max(a.starts[b], 0), a.capacity) : 0;
+    r.end = a.lens[b];
+    r.bad = r.end > a.capacity;
+    if (r.bad) r.end = 0;
+    r.units = max(1, (int)a.by_unit.div((uint32_t)(max(r.end - r.first, 0) + a.unit_tokens - 1)));
     return r;
+}
+
+// The parts of a segment of 8 * NT heads: `slots` of [heads][DMAX + 2] floats,
+// the last two the maximum and the sum.  Block c uses slot 2c for the segment
+// that holds its first unit and 2c + 1 for its last.
+template <int DMAX>
+__device__ __forceinline__ float* part_row(float* parts, int slot, int heads, int hh) {
+    return parts + ((int64_t)slot * heads + hh) * (DMAX + 4);
+}
+
+__device__ __forceinline__ void store_row(const AttArgs& a, int b, int head, int d, float y) {
+    const int64_t at = b * a.out_b + head * a.out_h + d;
+    if (a.q_type == CHM_FP16)
+        static_cast<__half*>(a.out)[at] = __float2half_rn(y);
+    else
+        static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
 }
 
 // DMAX: dim rounded up to 64, 128 or 256; NT: blocks of 8 query heads.
 template <int DMAX, int KIND, int NT>
-__global__ void __launch_bounds__(kAttThreads) paged_attention_kernel(const AttArgs a) {
-    constexpr bool kWide = KIND == CHM_FP16 || KIND == CHM_BF16;  // 16-bit cache
-    constexpr bool kHalf = KIND == CHM_FP16;                      // type of the products
+struct Shape {
+    static constexpr bool kWide = KIND == CHM_FP16 || KIND == CHM_BF16;  // 16-bit cache
+    static constexpr int kU = kWide ? 1 : 2;                             // groups of 16 tokens per warp and step
+    static constexpr int kTok = 16 * kU;
+    static constexpr int kTile = kAttWarps * kTok;
+    static constexpr int kHeads = 8 * NT;
+    // blocks per SM that the registers (K, V and output tiles) leave room for
+    static constexpr int kResident = DMAX <= 64 ? (NT == 1 ? 4 : 3) : DMAX <= 128 && NT == 1 ? 3 : 2;
+};
+
+template <int DMAX, int KIND, int NT>
+__global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
+    paged_attention_kernel(const AttArgs a) {
+    using S = Shape<DMAX, KIND, NT>;
+    constexpr bool kWide = S::kWide;
+    constexpr bool kHalf = KIND == CHM_FP16;  // type of the products
     constexpr int kBytes = kWide ? 2 : 1;
-    constexpr int kU = kWide ? 1 : 2;        // groups of 16 tokens per warp and step
-    constexpr int kTok = 16 * kU;
+    constexpr int kU = S::kU, kTok = S::kTok, kTile = S::kTile, kHeads = S::kHeads;
     constexpr int kKC = DMAX * kBytes / 64;  // 16-byte runs of a key per thread
-    constexpr int kSteps = DMAX / 16;        // products along dim
+    constexpr int kRuns = DMAX / 32;         // operand runs of q
     constexpr int kE = DMAX / 8;             // value elements per thread and token
     constexpr int kVC = kE * kBytes / 8;     // 8-byte runs of a value per thread
     constexpr int kM = kE / 2;               // 16-row blocks of the output
-    constexpr int kHeads = 8 * NT;
     constexpr int kRow = DMAX + 4;
-    __shared__ uint4 s_q[2][NT][kSteps / 2][32];  // high and low part of q as operand registers
-    __shared__ float s_o[kAttWarps][kHeads][kRow];
+    __shared__ uint4 s_q[2][NT][kRuns][32];  // high and low part of q as operand registers
+    __shared__ __align__(16) float s_o[kAttWarps][kHeads][kRow];
     __shared__ float s_m[kAttWarps][kHeads], s_l[kAttWarps][kHeads];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int seg = blockIdx.x, b = blockIdx.y;
-    const int head = seg / a.blocks;
-    const int h0 = head * a.group + (seg - head * a.blocks) * kHeads;  // first query head
-    const int nh = min(kHeads, (head + 1) * a.group - h0);
     const int dim = a.c.dim;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    Sequence s;
-    s.table = a.tables + b * a.table_stride;
-    s.first = a.starts ? min(max(a.starts[b], 0), a.capacity) : 0;
-    s.end = a.lens[b];
-    bool bad = s.end > a.capacity;
-    if (bad) s.end = 0;
-
-    // q: lane (g, t) of run i holds the 8 elements that its key runs meet
+    // ---- this block's units (every warp works them out for itself)
+    const int segs = a.c.heads * a.blocks;
+    int total = 0;
+    for (int b = lane; b < a.batch; b += 32) total += sequence_range(a, b).units;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
+    total *= segs;
+    const int per = (total + (int)gridDim.x - 1) / (int)gridDim.x;
+    int u = blockIdx.x * per;
+    const int u1 = min(u + per, total);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.plan = Plan{per, total};
+    if (u >= u1) return;
+    int b = 0, before = 0;  // the sequence that holds unit u, the units of those before it
+    for (int base = 0; base < a.batch; base += 32) {
+        const int n = base + lane < a.batch ? sequence_range(a, base + lane).units * segs : 0;
+        int sum = n;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, sum, x);
+            if (lane >= x) sum += y;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, base + lane < a.batch && before + sum > u);
+        if (past) {
+            const int at = __ffs(past) - 1;
+            b = base + at;
+            before += __shfl_sync(0xffffffffu, sum - n, at);
+            break;
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    Range r = sequence_range(a, b);
     const bool split_q = !kWide && a.q_type == CHM_FP16;
-    for (int i = threadIdx.x; i < NT * (kSteps / 2) * 32; i += kAttThreads) {
-        const int ln = i & 31, run = (i >> 5) % (kSteps / 2), nt = (i >> 5) / (kSteps / 2);
-        const int hh = nt * 8 + (ln >> 2);
-        const int d0 = kWide ? run * 32 + (ln & 3) * 8 : (run >> 1) * 64 + (ln & 3) * 16 + (run & 1) * 8;
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float x[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int d = d0 + 2 * j + e;
-                x[e] = 0.0f;
-                if (hh < nh && d < dim) {
-                    const int64_t at = b * a.q_b + (h0 + hh) * a.q_h + d;
-                    x[e] = a.q_type == CHM_FP16 ? __half2float(static_cast<const __half*>(a.q)[at])
-                                                : __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[at]);
+    const char* const kbase = static_cast<const char*>(a.c.k);
+    const char* const vbase = static_cast<const char*>(a.c.v);
+
+    for (int piece = 0; u < u1; ++piece) {
+        const int in_seq = u - before;
+        const int seg = in_seq / r.units;
+        const int unit0 = in_seq - seg * r.units;
+        const int unit1 = min(r.units, unit0 + (u1 - u));
+        const bool whole = unit1 - unit0 == r.units;
+        if (piece == 0 && threadIdx.x == 0) a.boundaries[blockIdx.x] = Boundary{b, seg, u - unit0, r.units};
+        const int head = seg / a.blocks;
+        const int h0 = head * a.group + (seg - head * a.blocks) * kHeads;  // first query head
+        const int nh = min(kHeads, (head + 1) * a.group - h0);
+        const int32_t* table = a.tables + b * a.table_stride;
+        const int first = r.first + unit0 * a.unit_tokens;
+        const int end = unit1 == r.units ? r.end : r.first + unit1 * a.unit_tokens;
+        bool bad = r.bad;
+
+        // Token `pos` of the range, one per lane: its page, then its place and scales.
+        auto page_of = [&](int pos) { return pos < end ? table[a.by_page.div((uint32_t)pos)] : 0; };
+        int64_t at = -1;  // element offset, -1: none
+        float ks = 0.0f, vs = 0.0f;
+        auto place = [&](int pos, int page) {
+            at = -1;
+            if (pos < end) {
+                if (page < 0 || page >= a.c.num_pages) {
+                    bad = true;
+                } else {
+                    const uint32_t within = (uint32_t)pos - a.by_page.div((uint32_t)pos) * (uint32_t)a.c.page_size;
+                    at = page * a.c.page_stride + (int64_t)head * a.c.head_stride +
+                         (int64_t)within * a.c.token_stride;
+                    if (!kWide) {
+                        const int64_t i = ((int64_t)page * a.c.heads + head) * a.c.page_size + within;
+                        ks = a.c.k_scale[i];
+                        vs = a.c.v_scale[i];
+                    }
                 }
             }
-            hi[j] = pack16<kHalf>(x[0], x[1]);
-            const float2 r = unpack16<kHalf>(hi[j]);
-            lo[j] = pack16<kHalf>(x[0] - r.x, x[1] - r.y);
+        };
+        uint4 kr[kU][2][kKC];
+        auto load_keys = [&]() {
+#pragma unroll
+            for (int i = 0; i < kU; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int64_t x = __shfl_sync(0xffffffffu, at, i * 16 + h * 8 + g);
+                    const char* p = kbase + x * kBytes + t * 16;
+#pragma unroll
+                    for (int c = 0; c < kKC; ++c) {
+                        kr[i][h][c] = make_uint4(0, 0, 0, 0);
+                        if (x >= 0 && c * 64 + t * 16 < dim * kBytes) kr[i][h][c] = ldg16(p + c * 64);
+                    }
+                }
+        };
+        uint32_t vr[kU][4][kVC * 2];
+        auto load_values = [&]() {
+#pragma unroll
+            for (int i = 0; i < kU; ++i)
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    const int64_t x = __shfl_sync(0xffffffffu, at, i * 16 + (h >> 1) * 8 + 2 * t + (h & 1));
+                    const char* p = vbase + x * kBytes;
+                    if (kVC >= 2) {
+#pragma unroll
+                        for (int c = 0; c < kVC / 2; ++c) {
+                            uint4 w = make_uint4(0, 0, 0, 0);
+                            const int off = c * 128 + g * 16;
+                            if (x >= 0 && off < dim * kBytes) w = ldg16(p + off);
+                            vr[i][h][c * 4] = w.x, vr[i][h][c * 4 + 1] = w.y;
+                            vr[i][h][c * 4 + 2] = w.z, vr[i][h][c * 4 + 3] = w.w;
+                        }
+                    } else {
+                        uint2 w = make_uint2(0, 0);
+                        if (x >= 0 && g * 8 < dim) w = ldg8(p + g * 8);
+                        vr[i][h][0] = w.x, vr[i][h][1] = w.y;
+                    }
+                }
+        };
+
+        int pos = first + warp * kTok + lane % kTok;  // this lane's token
+        int next_page = page_of(pos + kTile);
+        place(pos, page_of(pos));
+        load_keys();
+
+        // q: lane (g, t) of a run holds the 8 elements that its key runs meet
+        for (int i = threadIdx.x; i < NT * kRuns * 32; i += kAttThreads) {
+            const int ln = i & 31, run = (i >> 5) % kRuns, nt = (i >> 5) / kRuns;
+            const int hh = nt * 8 + (ln >> 2);
+            const int d0 = kWide ? run * 32 + (ln & 3) * 8 : (run >> 1) * 64 + (ln & 3) * 16 + (run & 1) * 8;
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float x[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int d = d0 + 2 * j + e;
+                    x[e] = 0.0f;
+                    if (hh < nh && d < dim) {
+                        const int64_t qa = b * a.q_b + (h0 + hh) * a.q_h + d;
+                        x[e] = a.q_type == CHM_FP16 ? __half2float(static_cast<const __half*>(a.q)[qa])
+                                                    : __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[qa]);
+                    }
+                }
+                hi[j] = pack16<kHalf>(x[0], x[1]);
+                const float2 y = unpack16<kHalf>(hi[j]);
+                lo[j] = pack16<kHalf>(x[0] - y.x, x[1] - y.y);
+            }
+            s_q[0][nt][run][ln] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            s_q[1][nt][run][ln] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
-        s_q[0][nt][run][ln] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        s_q[1][nt][run][ln] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    }
-    __syncthreads();
+        __syncthreads();
 
-    float o[NT][kM][4] = {};
-    float m[NT][2], l[NT][2];
+        float o[NT][kM][4] = {};
+        float m[NT][2], l[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.0f;
+        for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.0f;
 
-    for (int base = s.first + warp * kTok; base < s.end; base += kAttWarps * kTok) {
-        const TokenInfo info = token_info<KIND>(a, s, base + lane % kTok, head, bad);
-        // ---- scores
-        float sc[NT][kU][4] = {};
+        // Keys of a step are loaded a step ahead, its values before its scores
+        // are worked out, its pages two steps ahead.
+        for (int base = first + warp * kTok; base < end; base += kTile) {
+            load_values();
+            const float ks_now = ks, vs_now = vs;
+            const int page = next_page;
+            next_page = page_of(pos + 2 * kTile);
+            // ---- scores
+            float sc[NT][kU][4] = {};
 #pragma unroll
-        for (int u = 0; u < kU; ++u) {
-            uint4 kr[2][kKC];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int64_t at = __shfl_sync(0xffffffffu, info.at, u * 16 + r * 8 + g);
-                const char* p = static_cast<const char*>(a.c.k) + at * kBytes + t * 16;
+            for (int i = 0; i < kU; ++i)
 #pragma unroll
                 for (int c = 0; c < kKC; ++c) {
-                    kr[r][c] = make_uint4(0, 0, 0, 0);
-                    if (at >= 0 && (c * 64 + t * 16) < dim * kBytes) kr[r][c] = ldg16(p + c * 64);
-                }
-            }
+                    const uint32_t w0[4] = {kr[i][0][c].x, kr[i][0][c].y, kr[i][0][c].z, kr[i][0][c].w};
+                    const uint32_t w1[4] = {kr[i][1][c].x, kr[i][1][c].y, kr[i][1][c].z, kr[i][1][c].w};
+                    // pairs of the run: 4 words of a 16-bit cache, 8 pairs of codes
 #pragma unroll
-            for (int c = 0; c < kKC; ++c) {
-                const uint32_t w0[4] = {kr[0][c].x, kr[0][c].y, kr[0][c].z, kr[0][c].w};
-                const uint32_t w1[4] = {kr[1][c].x, kr[1][c].y, kr[1][c].z, kr[1][c].w};
-                // pairs of the run: 4 words of a 16-bit cache, 8 pairs of codes
+                    for (int j = 0; j < (kWide ? 1 : 2); ++j) {
+                        uint32_t p0[4], p1[4];
 #pragma unroll
-                for (int j = 0; j < (kWide ? 1 : 2); ++j) {
-                    uint32_t p0[4], p1[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (kWide) {
-                            p0[i] = w0[i], p1[i] = w1[i];
-                        } else {
-                            const uint32_t x0 = w0[j * 2 + (i >> 1)], x1 = w1[j * 2 + (i >> 1)];
-                            const uint32_t sel = KIND == CHM_INT8 ? ((i & 1) ? 0x4342 : 0x4140) : ((i & 1) ? 0x3424 : 0x1404);
-                            p0[i] = codes_to_bf16<KIND>(__byte_perm(x0, 0, sel));
-                            p1[i] = codes_to_bf16<KIND>(__byte_perm(x1, 0, sel));
+                        for (int e = 0; e < 4; ++e) {
+                            if (kWide) {
+                                p0[e] = w0[e], p1[e] = w1[e];
+                            } else {
+                                const uint32_t x0 = w0[j * 2 + (e >> 1)], x1 = w1[j * 2 + (e >> 1)];
+                                const uint32_t sel =
+                                    KIND == CHM_INT8 ? ((e & 1) ? 0x4342 : 0x4140) : ((e & 1) ? 0x3424 : 0x1404);
+                                p0[e] = codes_to_bf16<KIND>(__byte_perm(x0, 0, sel));
+                                p1[e] = codes_to_bf16<KIND>(__byte_perm(x1, 0, sel));
+                            }
                         }
-                    }
-                    const int run = kWide ? c : c * 2 + j;
+                        const int run = kWide ? c : c * 2 + j;
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        uint4 bq = s_q[0][n][run][lane];
-                        mma<kHalf>(sc[n][u], p0[0], p1[0], p0[1], p1[1], bq.x, bq.y);
-                        mma<kHalf>(sc[n][u], p0[2], p1[2], p0[3], p1[3], bq.z, bq.w);
-                        if (!kWide && split_q) {
-                            bq = s_q[1][n][run][lane];
-                            mma<kHalf>(sc[n][u], p0[0], p1[0], p0[1], p1[1], bq.x, bq.y);
-                            mma<kHalf>(sc[n][u], p0[2], p1[2], p0[3], p1[3], bq.z, bq.w);
+                        for (int n = 0; n < NT; ++n) {
+                            uint4 bq = s_q[0][n][run][lane];
+                            mma<kHalf>(sc[n][i], p0[0], p1[0], p0[1], p1[1], bq.x, bq.y);
+                            mma<kHalf>(sc[n][i], p0[2], p1[2], p0[3], p1[3], bq.z, bq.w);
+                            if (!kWide && split_q) {
+                                bq = s_q[1][n][run][lane];
+                                mma<kHalf>(sc[n][i], p0[0], p1[0], p0[1], p1[1], bq.x, bq.y);
+                                mma<kHalf>(sc[n][i], p0[2], p1[2], p0[3], p1[3], bq.z, bq.w);
+                            }
                         }
                     }
                 }
-            }
-        }
-        // ---- running maximum; it follows the scores only when one passes it by more than 2^8
-        float vs[kU][2];
-        bool above = false;
+            pos += kTile;
+            place(pos, page);
+            load_keys();
+            // ---- running maximum; it follows the scores only when one passes it by more than 2^8
+            float vscale[kU][2];
+            bool above = false;
 #pragma unroll
-        for (int u = 0; u < kU; ++u)
+            for (int i = 0; i < kU; ++i)
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int src = u * 16 + r * 8 + g;
-                const bool on = base + src < s.end;
-                float f = a.scale_log2;
-                if (!kWide) {
-                    f *= __shfl_sync(0xffffffffu, info.ks, src);
-                    vs[u][r] = __shfl_sync(0xffffffffu, info.vs, src);
+                for (int h = 0; h < 2; ++h) {
+                    const int src = i * 16 + h * 8 + g;
+                    const bool on = base + src < end;
+                    float f = a.scale_log2;
+                    if (!kWide) {
+                        f *= __shfl_sync(0xffffffffu, ks_now, src);
+                        const float y = __shfl_sync(0xffffffffu, vs_now, src);
+                        vscale[i][h] = on ? y : 0.0f;
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float& x = sc[n][i][h * 2 + e];
+                            x = on ? x * f : -INFINITY;
+                            above = above || x > m[n][e] + 8.0f;
+                        }
                 }
+            if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float& x = sc[n][u][r * 2 + e];
-                        x = on ? x * f : -INFINITY;
-                        above = above || x > m[n][e] + 8.0f;
+                        float top = m[n][e];
+#pragma unroll
+                        for (int i = 0; i < kU; ++i) top = fmaxf(top, fmaxf(sc[n][i][e], sc[n][i][2 + e]));
+#pragma unroll
+                        for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                        const float f = top == m[n][e] ? 1.0f : exp2_fast(m[n][e] - top);
+                        m[n][e] = top;
+                        l[n][e] *= f;
+#pragma unroll
+                        for (int i = 0; i < kM; ++i) o[n][i][e] *= f, o[n][i][2 + e] *= f;
                     }
             }
-        if (__any_sync(0xffffffffu, above)) {
+            // ---- probabilities as the operand of the second product
+            uint32_t ph[NT][kU][2], pl[NT][kU][2];
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n) {
+                const float m0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float top = m[n][e];
+                for (int i = 0; i < kU; ++i)
 #pragma unroll
-                    for (int u = 0; u < kU; ++u) top = fmaxf(top, fmaxf(sc[n][u][e], sc[n][u][2 + e]));
-#pragma unroll
-                    for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-                    const float f = top == m[n][e] ? 1.0f : exp2_fast(m[n][e] - top);
-                    m[n][e] = top;
-                    l[n][e] *= f;
-#pragma unroll
-                    for (int i = 0; i < kM; ++i) o[n][i][e] *= f, o[n][i][2 + e] *= f;
-                }
-        }
-        // ---- probabilities as the operand of the second product
-        uint32_t ph[NT][kU][2], pl[NT][kU][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const float m0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
-#pragma unroll
-            for (int u = 0; u < kU; ++u)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    float p0 = exp2_fast(sc[n][u][r * 2] - m0), p1 = exp2_fast(sc[n][u][r * 2 + 1] - m1);
-                    l[n][0] += p0, l[n][1] += p1;
-                    if (!kWide) p0 *= vs[u][r], p1 *= vs[u][r];
-                    const uint32_t hi = pack16<kHalf>(p0, p1);
-                    const float2 h = unpack16<kHalf>(hi);
-                    ph[n][u][r] = transpose8(hi);
-                    pl[n][u][r] = transpose8(pack16<kHalf>(p0 - h.x, p1 - h.y));
-                }
-        }
-        // ---- values
-#pragma unroll
-        for (int u = 0; u < kU; ++u) {
-            uint32_t vr[4][kVC * 2];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int64_t at = __shfl_sync(0xffffffffu, info.at, u * 16 + (i >> 1) * 8 + 2 * t + (i & 1));
-                const char* p = static_cast<const char*>(a.c.v) + at * kBytes;
-                if (kVC >= 2) {
-#pragma unroll
-                    for (int c = 0; c < kVC / 2; ++c) {
-                        uint4 x = make_uint4(0, 0, 0, 0);
-                        const int off = c * 128 + g * 16;
-                        if (at >= 0 && off < dim * kBytes) x = ldg16(p + off);
-                        vr[i][c * 4] = x.x, vr[i][c * 4 + 1] = x.y, vr[i][c * 4 + 2] = x.z, vr[i][c * 4 + 3] = x.w;
+                    for (int h = 0; h < 2; ++h) {
+                        float p0 = exp2_fast(sc[n][i][h * 2] - m0), p1 = exp2_fast(sc[n][i][h * 2 + 1] - m1);
+                        l[n][0] += p0, l[n][1] += p1;
+                        if (!kWide) p0 *= vscale[i][h], p1 *= vscale[i][h];
+                        const uint32_t hi = pack16<kHalf>(p0, p1);
+                        const float2 y = unpack16<kHalf>(hi);
+                        ph[n][i][h] = transpose8(hi);
+                        pl[n][i][h] = transpose8(pack16<kHalf>(p0 - y.x, p1 - y.y));
                     }
-                } else {
-                    uint2 x = make_uint2(0, 0);
-                    if (at >= 0 && g * 8 < dim) x = ldg8(p + g * 8);
-                    vr[i][0] = x.x, vr[i][1] = x.y;
-                }
             }
+            // ---- values
 #pragma unroll
-            for (int i = 0; i < kM; ++i) {
-                uint32_t f[4];
+            for (int i = 0; i < kU; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {  // row block r & 1, tokens r >> 1
-                    const int x = i + (r & 1) * kM;
-                    const uint32_t* v0 = vr[(r >> 1) * 2];
-                    const uint32_t* v1 = vr[(r >> 1) * 2 + 1];
-                    if (kWide) {
-                        f[r] = __byte_perm(v0[x / 2], v1[x / 2], (x & 1) ? 0x7632 : 0x5410);
-                    } else {
-                        const int e = x & 3;
-                        // the codes in the low (int8) or high (e4m3) bytes of the halves
-                        const uint32_t sel = KIND == CHM_INT8 ? (uint32_t)(e | (4 + e) << 8) : (uint32_t)(e << 4 | (4 + e) << 12);
-                        f[r] = codes_to_bf16<KIND>(__byte_perm(v0[x / 4], v1[x / 4], sel));
+                for (int j = 0; j < kM; ++j) {
+                    uint32_t f[4];
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {  // row block h & 1, tokens h >> 1
+                        const int x = j + (h & 1) * kM;
+                        const uint32_t* v0 = vr[i][(h >> 1) * 2];
+                        const uint32_t* v1 = vr[i][(h >> 1) * 2 + 1];
+                        if (kWide) {
+                            f[h] = __byte_perm(v0[x / 2], v1[x / 2], (x & 1) ? 0x7632 : 0x5410);
+                        } else {
+                            // the codes in the low (int8) or high (e4m3) bytes of the halves
+                            const int e = x & 3;
+                            const uint32_t sel =
+                                KIND == CHM_INT8 ? (uint32_t)(e | (4 + e) << 8) : (uint32_t)(e << 4 | (4 + e) << 12);
+                            f[h] = codes_to_bf16<KIND>(__byte_perm(v0[x / 4], v1[x / 4], sel));
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma<kHalf>(o[n][j], f[0], f[1], f[2], f[3], ph[n][i][0], ph[n][i][1]);
+                        mma<kHalf>(o[n][j], f[0], f[1], f[2], f[3], pl[n][i][0], pl[n][i][1]);
                     }
                 }
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    mma<kHalf>(o[n][i], f[0], f[1], f[2], f[3], ph[n][u][0], ph[n][u][1]);
-                    mma<kHalf>(o[n][i], f[0], f[1], f[2], f[3], pl[n][u][0], pl[n][u][1]);
-                }
-            }
         }
-    }
 
-    // ---- the warps' parts joined
-    bad = __syncthreads_or(bad);
+        // ---- the warps' parts joined
+        bad = __syncthreads_or(bad);
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            float sum = l[n][e];
+            for (int e = 0; e < 2; ++e) {
+                float sum = l[n][e];
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-            const int hh = n * 8 + 2 * t + e;
-            if (g == 0) s_m[warp][hh] = m[n][e], s_l[warp][hh] = sum;
+                for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+                const int hh = n * 8 + 2 * t + e;
+                if (g == 0) s_m[warp][hh] = m[n][e], s_l[warp][hh] = sum;
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-                for (int i = 0; i < kM; ++i) {
-                    const int x = i + half * kM;
+                for (int x = 0; x < kE; x += 4) {
                     const int d = kWide ? (x / 8) * 64 + g * 8 + x % 8
                                         : kE >= 16 ? (x / 16) * 128 + g * 16 + x % 16 : g * 8 + x;
-                    s_o[warp][hh][d] = o[n][i][half * 2 + e];
+                    const int j = x % kM, k = x / kM * 2 + e;
+                    *reinterpret_cast<float4*>(&s_o[warp][hh][d]) =
+                        make_float4(o[n][j][k], o[n][j + 1][k], o[n][j + 2][k], o[n][j + 3][k]);
                 }
-        }
-    __syncthreads();
-    for (int i = threadIdx.x; i < nh * dim; i += kAttThreads) {
-        const int hh = i / dim, d = i - hh * dim;
-        float top = -INFINITY;
+            }
+        __syncthreads();
+        for (int hh = warp; hh < nh; hh += kAttWarps) {
+            float top = -INFINITY, sum = 0.0f, f[kAttWarps];
 #pragma unroll
-        for (int w = 0; w < kAttWarps; ++w) top = fmaxf(top, s_m[w][hh]);
-        float sum = 0.0f, acc = 0.0f;
+            for (int w = 0; w < kAttWarps; ++w) top = fmaxf(top, s_m[w][hh]);
 #pragma unroll
-        for (int w = 0; w < kAttWarps; ++w) {
-            const float f = s_m[w][hh] == -INFINITY ? 0.0f : exp2_fast(s_m[w][hh] - top);
-            sum += f * s_l[w][hh];
-            acc += f * s_o[w][hh][d];
+            for (int w = 0; w < kAttWarps; ++w) {
+                f[w] = s_m[w][hh] == -INFINITY ? 0.0f : exp2_fast(s_m[w][hh] - top);
+                sum += f[w] * s_l[w][hh];
+            }
+            if (bad) sum = __int_as_float(0x7FC00000);
+            float* part = part_row<DMAX>(a.parts, 2 * blockIdx.x + (piece > 0), kHeads, hh);
+            for (int d = lane; d < dim; d += 32) {
+                float acc = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kAttWarps; ++w) acc += f[w] * s_o[w][hh][d];
+                if (whole)
+                    store_row(a, b, h0 + hh, d, sum == 0.0f ? 0.0f : bad ? sum : acc / sum);
+                else
+                    part[d] = acc;
+            }
+            if (lane == 0) {
+                if (!whole)
+                    part[DMAX] = top, part[DMAX + 1] = sum;
+                else if (a.lse)
+                    a.lse[(int64_t)b * a.q_heads + h0 + hh] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+            }
         }
-        float y = sum == 0.0f ? 0.0f : acc / sum;
-        float e = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
-        if (bad) y = e = __int_as_float(0x7FC00000);
-        const int64_t at = b * a.out_b + (h0 + hh) * a.out_h + d;
-        if (a.q_type == CHM_FP16)
-            static_cast<__half*>(a.out)[at] = __float2half_rn(y);
-        else
-            static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
-        if (d == 0 && a.lse) a.lse[(int64_t)b * a.q_heads + h0 + hh] = e;
+        u += unit1 - unit0;
+        if (u == before + r.units * segs && u < u1) {
+            before = u;
+            r = sequence_range(a, ++b);
+        }
     }
 }
+
+// Block (c, h): if the first segment of block c + 1 began in block c, head h of
+// that segment from its parts, in the order of the blocks.
+constexpr int kJoinThreads = 128;
+
+template <int DMAX, int NT>
+__global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const AttArgs a) {
+    constexpr int kHeads = 8 * NT;
+    constexpr int kWarps = kJoinThreads / 32;
+    constexpr int kV = DMAX / 32;  // elements per lane
+    __shared__ float s_acc[kWarps][DMAX];
+    __shared__ float s_top[kWarps], s_sum[kWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int per = a.plan->per;
+    const int c = blockIdx.x + 1;
+    if (c * (int64_t)per >= a.plan->total) return;
+    const Boundary s = a.boundaries[c];
+    const int c0 = s.first / per, c1 = (s.first + s.units - 1) / per;
+    if (s.first == c * per || c != c0 + 1) return;
+    const int head = s.seg / a.blocks;
+    const int h0 = head * a.group + (s.seg - head * a.blocks) * kHeads;
+    const int hh = blockIdx.y;
+    if (h0 + hh >= (head + 1) * a.group) return;
+    // each warp: every kWarps-th part, with a running maximum
+    float top = -INFINITY, sum = 0.0f, acc[kV] = {};
+#pragma unroll 4
+    for (int i = c0 + warp; i <= c1; i += kWarps) {
+        const int slot = 2 * i + (i == c0 && c0 * per != s.first);
+        const float* part = part_row<DMAX>(a.parts, slot, kHeads, hh);
+        const float m = part[DMAX], l = part[DMAX + 1];
+        const float now = fmaxf(top, m);
+        const float f = top == now ? 1.0f : exp2_fast(top - now);
+        const float w = m == -INFINITY ? 0.0f : exp2_fast(m - now);
+        top = now;
+        sum = sum * f + l * w;
+#pragma unroll
+        for (int v = 0; v < kV; ++v) acc[v] = acc[v] * f + part[v * 32 + lane] * w;
+    }
+#pragma unroll
+    for (int v = 0; v < kV; ++v) s_acc[warp][v * 32 + lane] = acc[v];
+    if (lane == 0) s_top[warp] = top, s_sum[warp] = sum;
+    __syncthreads();
+    top = -INFINITY, sum = 0.0f;
+    float f[kWarps];
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_top[w]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        f[w] = s_top[w] == -INFINITY ? 0.0f : exp2_fast(s_top[w] - top);
+        sum += f[w] * s_sum[w];
+    }
+    for (int d = threadIdx.x; d < a.c.dim; d += kJoinThreads) {
+        float y = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) y += f[w] * s_acc[w][d];
+        store_row(a, s.seq, h0 + hh, d, sum == 0.0f ? 0.0f : sum != sum ? sum : y / sum);
+    }
+    if (threadIdx.x == 0 && a.lse)
+        a.lse[(int64_t)s.seq * a.q_heads + h0 + hh] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+}
+
+static int sm_count() {
+    static int cached[64];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) {
+        cudaGetLastError();
+        return 148;
+    }
+    if (cached[dev] > 0) return cached[dev];
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+        cudaGetLastError();
+        return 148;
+    }
+    return cached[dev] = n;
+}
+
+struct Layout {
+    int blocks;       // thread blocks of the main kernel
+    int unit_tokens;  // tokens per unit
+    bool joins;       // whether a segment can be split
+};
 
 template <int DMAX, int KIND, int NT>
-static void launch_attention(AttArgs a, cudaStream_t st) {
-    a.blocks = (a.group + 8 * NT - 1) / (8 * NT);
-    const dim3 grid((unsigned)(a.c.heads * a.blocks), (unsigned)a.batch);
-    paged_attention_kernel<DMAX, KIND, NT><<<grid, kAttThreads, 0, st>>>(a);
+struct Launch {
+    using S = Shape<DMAX, KIND, NT>;
+
+    static Layout layout(const AttArgs& a) {
+        Layout y;
+        // up to 4 tiles a segment stays whole: a second launch costs more than they do
+        const int whole = 4 * S::kTile;
+        y.unit_tokens = a.capacity <= whole ? whole : S::kTile;
+        y.joins = a.capacity > whole;
+        const int64_t segs = (int64_t)a.c.heads * ((a.group + S::kHeads - 1) / S::kHeads);
+        const int64_t units = a.batch * segs * std::max<int64_t>(1, ((int64_t)a.capacity + y.unit_tokens - 1) / y.unit_tokens);
+        y.blocks = (int)std::min<int64_t>(units, (int64_t)sm_count() * S::kResident);
+        return y;
+    }
+    // Units are counted in 32 bits.
+    static bool fits(const AttArgs& a) {
+        const Layout y = layout(a);
+        const int64_t segs = (int64_t)a.c.heads * ((a.group + S::kHeads - 1) / S::kHeads);
+        const int64_t per_seq = std::max<int64_t>(1, ((int64_t)a.capacity + y.unit_tokens - 1) / y.unit_tokens);
+        return segs * per_seq <= (INT32_MAX - (1 << 16)) / std::max(1, a.batch);
+    }
+    template <typename A>
+    static void carve(A& arena, const Layout& y, AttArgs* a) {
+        auto plan = arena.template take<Plan>(1);
+        auto bounds = arena.template take<Boundary>(y.blocks);
+        auto parts = arena.template take<float>(y.joins ? (size_t)2 * y.blocks * S::kHeads * (DMAX + 4) : 0);
+        if (a) {
+            a->plan = (Plan*)plan;
+            a->boundaries = (Boundary*)bounds;
+            a->parts = (float*)parts;
+        }
+    }
+    static size_t workspace(const AttArgs& a) {
+        Counter c;
+        carve(c, layout(a), nullptr);
+        return c.s.off;
+    }
+    struct Counter {
+        Sizer s;
+        template <typename T>
+        void* take(size_t n) {
+            s.take<T>(n);
+            return nullptr;
+        }
+    };
+    static chm_status run(AttArgs a, void* ws, size_t ws_bytes, cudaStream_t st) {
+        const Layout y = layout(a);
+        Arena arena(ws, ws_bytes);
+        carve(arena, y, &a);
+        if (arena.overflow) return CHM_ERR_CAPACITY;
+        a.blocks = (a.group + S::kHeads - 1) / S::kHeads;
+        a.unit_tokens = y.unit_tokens;
+        a.by_unit = FastDiv((uint32_t)y.unit_tokens);
+        paged_attention_kernel<DMAX, KIND, NT><<<(unsigned)y.blocks, kAttThreads, 0, st>>>(a);
+        CHM_TRY(launch_status("paged_attention_kernel"));
+        if (!y.joins || y.blocks < 2) return CHM_OK;
+        // The join's blocks start while the main kernel's last ones run, and wait for its end.
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)(y.blocks - 1), (unsigned)std::min(S::kHeads, a.group));
+        cfg.blockDim = dim3(kJoinThreads);
+        cfg.stream = st;
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        CHM_CUDA(cudaLaunchKernelEx(&cfg, attention_join_kernel<DMAX, NT>, (const AttArgs)a));
+        return CHM_OK;
+    }
+};
+
+// Calls f on the Launch<> for a cache's type, dim and sharing.  More than 8
+// query heads per key head take two blocks of 8 at a time, so that up to 16
+// read the cache once; at dim 256 the registers hold one block.
+template <int KIND, typename F>
+static auto with_kind(const AttArgs& a, F f) {
+    if (a.c.dim > 128) return f(Launch<256, KIND, 1>{});
+    if (a.c.dim > 64) return a.group > 8 ? f(Launch<128, KIND, 2>{}) : f(Launch<128, KIND, 1>{});
+    return a.group > 8 ? f(Launch<64, KIND, 2>{}) : f(Launch<64, KIND, 1>{});
 }
 
-template <int KIND>
-static void dispatch_dim(const AttArgs& a, cudaStream_t st) {
-    // more than 8 query heads per key head take two blocks of 8 at a time, so
-    // that up to 16 read the cache once; at dim 256 the registers hold one block
-    if (a.c.dim > 128) return launch_attention<256, KIND, 1>(a, st);
-    if (a.c.dim > 64) {
-        if (a.group > 8) return launch_attention<128, KIND, 2>(a, st);
-        return launch_attention<128, KIND, 1>(a, st);
+template <typename F>
+static auto with_launch(const AttArgs& a, F f) {
+    switch (a.c.type) {
+        case CHM_FP16: return with_kind<CHM_FP16>(a, f);
+        case CHM_BF16: return with_kind<CHM_BF16>(a, f);
+        case CHM_INT8: return with_kind<CHM_INT8>(a, f);
+        default: return with_kind<CHM_E4M3>(a, f);
     }
-    if (a.group > 8) return launch_attention<64, KIND, 2>(a, st);
-    return launch_attention<64, KIND, 1>(a, st);
 }
 
 static chm_status refuse_attention(const char* why) {
@@ -451,8 +737,17 @@ static chm_status refuse_attention(const char* why) {
 
 extern "C" size_t chm_paged_attention_workspace_bytes(const chm_kv_cache* cache, int64_t batch, int32_t q_heads,
                                                       int32_t table_width) {
-    (void)cache, (void)batch, (void)q_heads, (void)table_width;
-    return 256;
+    using namespace chm;
+    if (check_cache(cache, "paged_attention") != CHM_OK) return 0;
+    if (batch < 0 || batch > 65535 || q_heads < 1 || q_heads % cache->heads || table_width < 0 ||
+        (int64_t)table_width * cache->page_size > (1 << 30))
+        return 0;
+    AttArgs a{};
+    a.c = *cache;
+    a.batch = (int32_t)batch;
+    a.group = q_heads / cache->heads;
+    a.capacity = table_width * cache->page_size;
+    return with_launch(a, [&](auto l) { return l.workspace(a); });
 }
 
 extern "C" chm_status chm_paged_attention(const chm_kv_cache* cache, const chm_heads* q, const chm_heads* out,
@@ -473,8 +768,6 @@ extern "C" chm_status chm_paged_attention(const chm_kv_cache* cache, const chm_h
     if ((int64_t)table_width * cache->page_size > (1 << 30)) return refuse_attention("a table spans at most 2^30 tokens");
     if (batch == 0) return CHM_OK;
     if (!q->data || !out->data || !lens || (table_width > 0 && !tables)) return refuse_attention("null pointer");
-    if (!workspace || workspace_bytes < chm_paged_attention_workspace_bytes(cache, batch, q->heads, table_width))
-        return CHM_ERR_CAPACITY;
     AttArgs a{};
     a.c = *cache;
     a.q = q->data;
@@ -493,11 +786,6 @@ extern "C" chm_status chm_paged_attention(const chm_kv_cache* cache, const chm_h
     a.lse = lse;
     a.by_page = FastDiv((uint32_t)cache->page_size);
     cudaStream_t st = (cudaStream_t)stream;
-    switch (cache->type) {
-        case CHM_FP16: dispatch_dim<CHM_FP16>(a, st); break;
-        case CHM_BF16: dispatch_dim<CHM_BF16>(a, st); break;
-        case CHM_INT8: dispatch_dim<CHM_INT8>(a, st); break;
-        default: dispatch_dim<CHM_E4M3>(a, st); break;
-    }
-    return launch_status("paged_attention_kernel");
+    if (!with_launch(a, [&](auto l) { return l.fits(a); })) return refuse_attention("too much work for one call");
+    return with_launch(a, [&](auto l) { return l.run(a, workspace, workspace_bytes, st); });
 }

@@ -449,7 +449,9 @@ chm_status chm_cache_read(const chm_kv_cache* cache, const int64_t* slots, int64
  * the range are not read.  A page id outside the cache that the range needs,
  * or a length past the table's end, makes the sequence's rows and lse NaN.
  * Softmax statistics and sums are fp32; probabilities enter the value product
- * as two 16-bit terms (high and remainder).  Results do not depend on timing.
+ * as two 16-bit terms (high and remainder).  A sequence may be cut elsewhere in
+ * another batch or with a wider table, which moves the rounding of its sums;
+ * the same call gives the same bits every time.
  * table_width * page_size is at most 2^30, batch 65,535.  Calls on one
  * workspace must not overlap. */
 size_t chm_paged_attention_workspace_bytes(const chm_kv_cache* cache, int64_t batch, int32_t q_heads,
