@@ -10,7 +10,9 @@
 // query heads of one key head as the 8 columns:
 //   S^T [tokens x heads] = K [tokens x dim] Q^T,   O^T [dim x heads] += V^T P^T.
 // Both contractions may take their index in any order, so a thread's 16-byte
-// loads are its operand registers as they come: no shared memory, no barrier.
+// runs are its operand registers as they come: each lane copies its own runs
+// into a ring of its own in shared memory, steps ahead, and reads them back;
+// no layout to swizzle, no barrier.
 #include <algorithm>
 #include <cmath>
 #include <cstdio>
@@ -50,18 +52,20 @@ struct AttArgs {
     FastDiv by_page;
 };
 
-__device__ __forceinline__ uint4 ldg16(const void* p) {
-    uint4 r;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-                 : "l"(p));
-    return r;
+// Asynchronous copies of N bytes into shared memory; zeros where `on` is false.
+template <int N>
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from, bool on) {
+    const int bytes = on ? N : 0;
+    if (N == 16)
+        asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(N), "r"(bytes) : "memory");
 }
-
-__device__ __forceinline__ uint2 ldg8(const void* p) {
-    uint2 r;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
-    return r;
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Until all but the newest N groups of this thread's copies have landed.
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 template <bool HALF>
@@ -182,12 +186,27 @@ __device__ __forceinline__ void store_row(const AttArgs& a, int b, int head, int
 template <int DMAX, int KIND, int NT>
 struct Shape {
     static constexpr bool kWide = KIND == CHM_FP16 || KIND == CHM_BF16;  // 16-bit cache
-    static constexpr int kU = kWide ? 1 : 2;                             // groups of 16 tokens per warp and step
+    static constexpr int kBytes = kWide ? 2 : 1;
+    static constexpr int kU = DMAX * kBytes <= 128 ? 2 : 1;  // groups of 16 tokens per warp and step
     static constexpr int kTok = 16 * kU;
     static constexpr int kTile = kAttWarps * kTok;
     static constexpr int kHeads = 8 * NT;
-    // blocks per SM that the registers (K, V and output tiles) leave room for
-    static constexpr int kResident = DMAX <= 64 ? (NT == 1 ? 4 : 3) : DMAX <= 128 && NT == 1 ? 3 : 2;
+    // blocks per SM that the registers (the output tiles) leave room for
+    static constexpr int kResident = DMAX * kBytes > 256 ? 1 : DMAX > 128 || NT > 1 ? 2 : 3;
+    // A warp's copies in flight: kStages steps of keys and of values, which fill
+    // the shared memory that the resident blocks have, about 190 KB per SM.
+    static constexpr int kSlot = kTok * DMAX * kBytes;
+    static constexpr int kStages = (kResident == 3 ? 8192 : kResident == 2 ? 12288 : 16384) / kSlot;
+    // shared memory: q as operand registers (high and low part), rings, scales;
+    // at a segment's end the warps' parts take the place of the rings
+    static constexpr int kQ = 2 * NT * (DMAX / 32) * 512;
+    static constexpr int kRing = kAttWarps * kStages * 2 * kSlot;
+    static constexpr int kScales = kWide ? 0 : kAttWarps * kStages * 2 * kTok * 4;
+    static constexpr int kRow = DMAX + 4;
+    static constexpr int kOut = kAttWarps * kHeads * (kRow + 2) * 4;
+    static_assert(kOut <= kRing, "the warps' parts fit in the rings");
+    static constexpr int kShared = kQ + kRing + kScales;
+    static_assert(kResident * (kShared + 1024) <= 227 * 1024, "the resident blocks' shared memory");
 };
 
 template <int DMAX, int KIND, int NT>
@@ -196,19 +215,30 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
     using S = Shape<DMAX, KIND, NT>;
     constexpr bool kWide = S::kWide;
     constexpr bool kHalf = KIND == CHM_FP16;  // type of the products
-    constexpr int kBytes = kWide ? 2 : 1;
-    constexpr int kU = S::kU, kTok = S::kTok, kTile = S::kTile, kHeads = S::kHeads;
-    constexpr int kKC = DMAX * kBytes / 64;  // 16-byte runs of a key per thread
-    constexpr int kRuns = DMAX / 32;         // operand runs of q
-    constexpr int kE = DMAX / 8;             // value elements per thread and token
-    constexpr int kVC = kE * kBytes / 8;     // 8-byte runs of a value per thread
-    constexpr int kM = kE / 2;               // 16-row blocks of the output
-    constexpr int kRow = DMAX + 4;
-    __shared__ uint4 s_q[2][NT][kRuns][32];  // high and low part of q as operand registers
-    __shared__ __align__(16) float s_o[kAttWarps][kHeads][kRow];
-    __shared__ float s_m[kAttWarps][kHeads], s_l[kAttWarps][kHeads];
+    constexpr int kBytes = S::kBytes, kU = S::kU, kTok = S::kTok, kTile = S::kTile, kHeads = S::kHeads;
+    constexpr int kStages = S::kStages, kSlot = S::kSlot;
+    constexpr int kKC = DMAX * kBytes / 64;     // 16-byte runs of a key per thread
+    constexpr int kRuns = DMAX / 32;            // operand runs of q
+    constexpr int kE = DMAX / 8;                // value elements per thread and token
+    constexpr int kVB = kE * kBytes < 16 ? 8 : 16;  // bytes of a run of a value
+    constexpr int kVC = kE * kBytes / kVB;      // runs of a value per thread
+    constexpr int kM = kE / 2;                  // 16-row blocks of the output
+    constexpr int kRow = S::kRow;
+    static_assert(S::kResident >= 1 && kStages >= 1, "shape");
+    extern __shared__ __align__(16) uint8_t smem[];
+    uint4(*s_q)[NT][kRuns][32] = reinterpret_cast<uint4(*)[NT][kRuns][32]>(smem);
+    float(*s_o)[kHeads][kRow] = reinterpret_cast<float(*)[kHeads][kRow]>(smem + S::kQ);
+    float(*s_m)[kHeads] = reinterpret_cast<float(*)[kHeads]>(smem + S::kQ + kAttWarps * kHeads * kRow * 4);
+    float(*s_l)[kHeads] = s_m + kAttWarps;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int dim = a.c.dim;
+    // This warp's ring: per stage the keys' runs, then the values', each lane's
+    // own 16 bytes in a row of 512, so that a lane reads back what it copied.
+    const uint8_t* const ring = smem + S::kQ + warp * (kStages * 2 * kSlot);
+    const float* const scales = reinterpret_cast<const float*>(smem + S::kQ + S::kRing) + warp * (kStages * 2 * kTok);
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
+    const uint32_t ring_v = (uint32_t)__cvta_generic_to_shared(ring) + lane * kVB;
+    const uint32_t scales_at = (uint32_t)__cvta_generic_to_shared(scales) + lane * 4;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     // ---- this block's units (every warp works them out for itself)
@@ -263,10 +293,10 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
 
         // Token `pos` of the range, one per lane: its page, then its place and scales.
         auto page_of = [&](int pos) { return pos < end ? table[a.by_page.div((uint32_t)pos)] : 0; };
-        int64_t at = -1;  // element offset, -1: none
-        float ks = 0.0f, vs = 0.0f;
-        auto place = [&](int pos, int page) {
+        int64_t at = -1;  // element offset of this lane's token of the newest step, -1: none
+        auto place = [&](int pos, int page, int stage) {
             at = -1;
+            int64_t scale = -1;
             if (pos < end) {
                 if (page < 0 || page >= a.c.num_pages) {
                     bad = true;
@@ -274,58 +304,66 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
                     const uint32_t within = (uint32_t)pos - a.by_page.div((uint32_t)pos) * (uint32_t)a.c.page_size;
                     at = page * a.c.page_stride + (int64_t)head * a.c.head_stride +
                          (int64_t)within * a.c.token_stride;
-                    if (!kWide) {
-                        const int64_t i = ((int64_t)page * a.c.heads + head) * a.c.page_size + within;
-                        ks = a.c.k_scale[i];
-                        vs = a.c.v_scale[i];
-                    }
+                    if (!kWide) scale = ((int64_t)page * a.c.heads + head) * a.c.page_size + within;
                 }
             }
+            if (!kWide && lane < kTok) {
+                const int64_t x = max(scale, (int64_t)0);
+                copy_async<4>(scales_at + stage * (2 * kTok * 4), a.c.k_scale + x, scale >= 0);
+                copy_async<4>(scales_at + stage * (2 * kTok * 4) + kTok * 4, a.c.v_scale + x, scale >= 0);
+            }
         };
-        uint4 kr[kU][2][kKC];
-        auto load_keys = [&]() {
+        auto copy_keys = [&](int stage) {
+            const uint32_t to = ring_at + stage * 2 * kSlot;
 #pragma unroll
             for (int i = 0; i < kU; ++i)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int64_t x = __shfl_sync(0xffffffffu, at, i * 16 + h * 8 + g);
-                    const char* p = kbase + x * kBytes + t * 16;
+                    const char* p = kbase + max(x, (int64_t)0) * kBytes + t * 16;
 #pragma unroll
                     for (int c = 0; c < kKC; ++c) {
-                        kr[i][h][c] = make_uint4(0, 0, 0, 0);
-                        if (x >= 0 && c * 64 + t * 16 < dim * kBytes) kr[i][h][c] = ldg16(p + c * 64);
+                        const bool in = c * 64 + t * 16 < dim * kBytes;
+                        copy_async<16>(to + ((i * 2 + h) * kKC + c) * 512, in ? p + c * 64 : p, x >= 0 && in);
                     }
                 }
         };
-        uint32_t vr[kU][4][kVC * 2];
-        auto load_values = [&]() {
+        auto copy_values = [&](int stage) {
+            const uint32_t to = ring_v + stage * 2 * kSlot + kSlot;
 #pragma unroll
             for (int i = 0; i < kU; ++i)
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
                     const int64_t x = __shfl_sync(0xffffffffu, at, i * 16 + (h >> 1) * 8 + 2 * t + (h & 1));
-                    const char* p = vbase + x * kBytes;
-                    if (kVC >= 2) {
+                    const char* p = vbase + max(x, (int64_t)0) * kBytes;
 #pragma unroll
-                        for (int c = 0; c < kVC / 2; ++c) {
-                            uint4 w = make_uint4(0, 0, 0, 0);
-                            const int off = c * 128 + g * 16;
-                            if (x >= 0 && off < dim * kBytes) w = ldg16(p + off);
-                            vr[i][h][c * 4] = w.x, vr[i][h][c * 4 + 1] = w.y;
-                            vr[i][h][c * 4 + 2] = w.z, vr[i][h][c * 4 + 3] = w.w;
-                        }
-                    } else {
-                        uint2 w = make_uint2(0, 0);
-                        if (x >= 0 && g * 8 < dim) w = ldg8(p + g * 8);
-                        vr[i][h][0] = w.x, vr[i][h][1] = w.y;
+                    for (int c = 0; c < kVC; ++c) {
+                        const int off = c * 128 + g * kVB;
+                        const bool in = off < dim * kBytes;
+                        copy_async<kVB>(to + ((i * 4 + h) * kVC + c) * (32 * kVB), in ? p + off : p, x >= 0 && in);
                     }
                 }
         };
 
-        int pos = first + warp * kTok + lane % kTok;  // this lane's token
-        int next_page = page_of(pos + kTile);
-        place(pos, page_of(pos));
-        load_keys();
+        int pos = first + warp * kTok + lane % kTok;  // this lane's token of the newest step
+        int base = first + warp * kTok;               // the oldest step's first
+        int next_page = page_of(pos);
+#pragma unroll
+        for (int i = 0; i < kStages; ++i) {
+            const int page = next_page;
+            next_page = page_of(pos + kTile);
+            if (base + i * kTile < end) {
+                place(pos, page, i);
+                copy_keys(i);
+                copies_commit();
+                copy_values(i);
+                copies_commit();
+            } else {
+                copies_commit();
+                copies_commit();
+            }
+            pos += kTile;
+        }
 
         // q: lane (g, t) of a run holds the 8 elements that its key runs meet
         for (int i = threadIdx.x; i < NT * kRuns * 32; i += kAttThreads) {
@@ -360,21 +398,26 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
 #pragma unroll
         for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.0f;
 
-        // Keys of a step are loaded a step ahead, its values before its scores
-        // are worked out, its pages two steps ahead.
-        for (int base = first + warp * kTok; base < end; base += kTile) {
-            load_values();
-            const float ks_now = ks, vs_now = vs;
+        // The copies run kStages steps ahead: a step's keys and values are copied into the
+        // slots that the step kStages before it has just been read from.
+        int stage = 0;
+        for (; base < end; base += kTile) {
+            const uint8_t* const keys = ring + stage * 2 * kSlot + lane * 16;
+            const uint8_t* const values = ring + stage * 2 * kSlot + kSlot + lane * kVB;
+            const bool more = base + kStages * kTile < end;
             const int page = next_page;
-            next_page = page_of(pos + 2 * kTile);
+            next_page = page_of(pos + kTile);
+            copies_wait<2 * kStages - 1>();
+            __syncwarp();
             // ---- scores
             float sc[NT][kU][4] = {};
 #pragma unroll
             for (int i = 0; i < kU; ++i)
 #pragma unroll
                 for (int c = 0; c < kKC; ++c) {
-                    const uint32_t w0[4] = {kr[i][0][c].x, kr[i][0][c].y, kr[i][0][c].z, kr[i][0][c].w};
-                    const uint32_t w1[4] = {kr[i][1][c].x, kr[i][1][c].y, kr[i][1][c].z, kr[i][1][c].w};
+                    const uint4 r0 = *reinterpret_cast<const uint4*>(keys + (i * 2 * kKC + c) * 512);
+                    const uint4 r1 = *reinterpret_cast<const uint4*>(keys + ((i * 2 + 1) * kKC + c) * 512);
+                    const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
                     // pairs of the run: 4 words of a 16-bit cache, 8 pairs of codes
 #pragma unroll
                     for (int j = 0; j < (kWide ? 1 : 2); ++j) {
@@ -405,9 +448,6 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
                         }
                     }
                 }
-            pos += kTile;
-            place(pos, page);
-            load_keys();
             // ---- running maximum; it follows the scores only when one passes it by more than 2^8
             float vscale[kU][2];
             bool above = false;
@@ -419,9 +459,8 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
                     const bool on = base + src < end;
                     float f = a.scale_log2;
                     if (!kWide) {
-                        f *= __shfl_sync(0xffffffffu, ks_now, src);
-                        const float y = __shfl_sync(0xffffffffu, vs_now, src);
-                        vscale[i][h] = on ? y : 0.0f;
+                        f *= scales[stage * 2 * kTok + src];
+                        vscale[i][h] = scales[stage * 2 * kTok + kTok + src];
                     }
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
@@ -432,6 +471,13 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
                             above = above || x > m[n][e] + 8.0f;
                         }
                 }
+            if (!kWide) __syncwarp();  // the scales are read; the next step's take their place
+            if (more) {
+                place(pos, page, stage);
+                copy_keys(stage);
+            }
+            copies_commit();
+            pos += kTile;
             if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
@@ -468,16 +514,31 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
                     }
             }
             // ---- values
+            copies_wait<2 * kStages - 1>();
 #pragma unroll
-            for (int i = 0; i < kU; ++i)
+            for (int i = 0; i < kU; ++i) {
+                uint32_t vr[4][kVC * kVB / 4];
+#pragma unroll
+                for (int h = 0; h < 4; ++h)
+#pragma unroll
+                    for (int c = 0; c < kVC; ++c) {
+                        const uint8_t* x = values + ((i * 4 + h) * kVC + c) * (32 * kVB);
+                        if (kVB == 16) {
+                            const uint4 w = *reinterpret_cast<const uint4*>(x);
+                            vr[h][c * 4] = w.x, vr[h][c * 4 + 1] = w.y, vr[h][c * 4 + 2] = w.z, vr[h][c * 4 + 3] = w.w;
+                        } else {
+                            const uint2 w = *reinterpret_cast<const uint2*>(x);
+                            vr[h][0] = w.x, vr[h][1] = w.y;
+                        }
+                    }
 #pragma unroll
                 for (int j = 0; j < kM; ++j) {
                     uint32_t f[4];
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {  // row block h & 1, tokens h >> 1
                         const int x = j + (h & 1) * kM;
-                        const uint32_t* v0 = vr[i][(h >> 1) * 2];
-                        const uint32_t* v1 = vr[i][(h >> 1) * 2 + 1];
+                        const uint32_t* v0 = vr[(h >> 1) * 2];
+                        const uint32_t* v1 = vr[(h >> 1) * 2 + 1];
                         if (kWide) {
                             f[h] = __byte_perm(v0[x / 2], v1[x / 2], (x & 1) ? 0x7632 : 0x5410);
                         } else {
@@ -494,7 +555,12 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
                         mma<kHalf>(o[n][j], f[0], f[1], f[2], f[3], pl[n][i][0], pl[n][i][1]);
                     }
                 }
+            }
+            if (more) copy_values(stage);
+            copies_commit();
+            stage = stage + 1 == kStages ? 0 : stage + 1;
         }
+        copies_wait<0>();
 
         // ---- the warps' parts joined
         bad = __syncthreads_or(bad);
@@ -544,6 +610,7 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
                     a.lse[(int64_t)b * a.q_heads + h0 + hh] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
             }
         }
+        __syncthreads();  // the parts are read; the next segment's copies take their place
         u += unit1 - unit0;
         if (u == before + r.units * segs && u < u1) {
             before = u;
@@ -688,7 +755,15 @@ struct Launch {
         a.blocks = (a.group + S::kHeads - 1) / S::kHeads;
         a.unit_tokens = y.unit_tokens;
         a.by_unit = FastDiv((uint32_t)y.unit_tokens);
-        paged_attention_kernel<DMAX, KIND, NT><<<(unsigned)y.blocks, kAttThreads, 0, st>>>(a);
+        static bool set[64];  // per device: the kernel may take this much shared memory
+        int dev = 0;
+        CHM_CUDA(cudaGetDevice(&dev));
+        if (dev >= 64 || !set[dev]) {
+            CHM_CUDA(cudaFuncSetAttribute(paged_attention_kernel<DMAX, KIND, NT>,
+                                          cudaFuncAttributeMaxDynamicSharedMemorySize, S::kShared));
+            if (dev < 64) set[dev] = true;
+        }
+        paged_attention_kernel<DMAX, KIND, NT><<<(unsigned)y.blocks, kAttThreads, S::kShared, st>>>(a);
         CHM_TRY(launch_status("paged_attention_kernel"));
         if (!y.joins || y.blocks < 2) return CHM_OK;
         // The join's blocks start while the main kernel's last ones run, and wait for its end.
