@@ -156,9 +156,14 @@ __global__ void __launch_bounds__(kCacheThreads) cache_read_kernel(const CacheAr
             const float s = (side ? a.c.v_scale : a.c.k_scale)[(page * a.c.heads + h) * a.c.page_size + within];
             const uint2 w = *reinterpret_cast<const uint2*>(base + at);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t byte = ((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 0xFFu;
-                x[i] = (KIND == CHM_INT8 ? (float)(int8_t)byte : e4m3_value(byte)) * s;
+            for (int i = 0; i < 8; i += 2) {
+                const uint32_t two = ((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 0xFFFFu;
+                float2 y;
+                if (KIND == CHM_INT8)
+                    y = make_float2((float)(int8_t)(two & 0xFFu), (float)(int8_t)(two >> 8));
+                else
+                    y = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3)));
+                x[i] = y.x * s, x[i + 1] = y.y * s;
             }
         }
     }

@@ -1,6 +1,8 @@
 // The paged key-value cache as the kernels see it, and its 8-bit codes.
 #pragma once
 
+#include <cstdio>
+
 #include "vectors.cuh"
 
 namespace chm {
@@ -21,6 +23,7 @@ inline chm_status check_cache(const chm_kv_cache* c, const char* who) {
     if (c->num_pages > (INT64_MAX >> 8) / c->page_size / c->heads) return bad("too many pages");
     if (c->dim < 16 || c->dim > 256 || c->dim % 16) return bad("dim must be a multiple of 16, at most 256");
     const int run = 16 / type_bytes(c->type);
+    if (c->page_stride < 0 || c->head_stride < 0 || c->token_stride < 0) return bad("cache strides must not be negative");
     if (c->page_stride % run || c->head_stride % run || c->token_stride % run)
         return bad("cache strides must be multiples of 16 bytes");
     if (!aligned16(c->k) || !aligned16(c->v)) return bad("cache memory must be 16-byte aligned");
@@ -28,14 +31,6 @@ inline chm_status check_cache(const chm_kv_cache* c, const char* who) {
     if (c->num_pages > 0 && (!c->k || !c->v)) return bad("null pages");
     if (c->num_pages > 0 && scaled && (!c->k_scale || !c->v_scale)) return bad("an 8-bit cache needs its scales");
     return CHM_OK;
-}
-
-// e4m3 (sign, 4 exponent bits with bias 7, 3 fraction bits) as fp32: the bits
-// sit 20 to the left as an fp32 whose exponent is 120 too low; subnormal codes
-// become subnormal fp32 numbers and come out of the product exactly.
-__device__ __forceinline__ float e4m3_value(uint32_t byte) {
-    const float x = __uint_as_float((byte & 0x7Fu) << 20) * 1.329227995784915872903807060280344576e36f;  // 2^120
-    return (byte & 0x80u) ? -x : x;
 }
 
 }  // namespace chm

@@ -17,6 +17,8 @@
 #include <cmath>
 #include <cstdio>
 
+#include <cuda_fp8.h>
+
 #include "kv_cache.cuh"
 
 namespace chm {
@@ -25,39 +27,57 @@ constexpr int kAttWarps = 4;
 constexpr int kAttThreads = kAttWarps * 32;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
+constexpr uint32_t kNowhere = 0xFFFFFFFFu;
 
-struct Plan;
-struct Boundary;
+struct Plan {
+    int per;    // units per block
+    int total;  // units
+};
+struct Boundary {  // the segment that holds a block's first unit
+    int seq, seg;
+    int first, units;  // its first unit, its units
+};
 
 struct AttArgs {
     chm_kv_cache c;
+    uint32_t page16, head16, token16;  // the cache's strides in 16 bytes
     const void* q;
     void* out;
     int64_t q_b, q_h, out_b, out_h;
     int32_t q_type;
+    bool q_wide;                    // q in 16-byte loads
     int32_t batch, q_heads, group;  // group: query heads per key head
     int32_t blocks;                 // blocks of 8 * NT query heads per key head
     const int32_t* tables;
     int64_t table_stride;
     int32_t capacity;     // table_width * page_size
     int32_t unit_tokens;  // tokens per unit of work
-    FastDiv by_unit;
-    Plan* plan;
-    Boundary* boundaries;
-    float* parts;
+    FastDiv by_unit, by_page;
     const int32_t* lens;
     const int32_t* starts;
     float scale_log2;
     float* lse;
-    FastDiv by_page;
+    Plan* plan;
+    int32_t* before;  // units before each sequence
+    Boundary* boundaries;
+    float* parts;
+    bool join_segments;  // the join's blocks stand for segments, not boundaries
 };
 
-// Asynchronous copies of N bytes into shared memory; zeros where `on` is false.
+// Asynchronous copies of N bytes into shared memory, `OFF` bytes past `from`;
+// the second form writes zeros where `on` is false.
+template <int N, int OFF>
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
+    if (N == 16)
+        asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1 + %2], 16;" ::"r"(to), "l"(from), "n"(OFF) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1 + %2], %3;" ::"r"(to), "l"(from), "n"(OFF), "n"(N) : "memory");
+}
 template <int N>
-__device__ __forceinline__ void copy_async(uint32_t to, const void* from, bool on) {
+__device__ __forceinline__ void copy_async_if(uint32_t to, const void* from, bool on) {
     const int bytes = on ? N : 0;
     if (N == 16)
-        asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
     else
         asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(N), "r"(bytes) : "memory");
 }
@@ -90,9 +110,15 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     return r;
 }
 
+// 2^x, log2 x; results below 2^-126 are zero.
 __device__ __forceinline__ float exp2_fast(float x) {
     float r;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float log2_fast(float x) {
+    float r;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 
@@ -112,43 +138,49 @@ __device__ __forceinline__ float2 unpack16(uint32_t x) {
     return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u));
 }
 
-// Two 8-bit codes as bf16 pairs, exactly.  int8: `y` holds the codes in the
-// low bytes of its halves; 128 + (code & 127) less 128, or 256 for a negative
-// code.  e4m3: the codes in the high bytes; a bf16 with an exponent 120 too
-// low, times 2^120 (subnormal codes come out of the product exactly too).
-template <int KIND>
-__device__ __forceinline__ uint32_t codes_to_bf16(uint32_t y) {
-    __nv_bfloat162 r;
-    if (KIND == CHM_INT8) {
-        const uint32_t a = (y & 0x007F007Fu) | 0x43004300u;
-        const uint32_t b = (y & 0x00800080u) | 0x43004300u;
-        r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-    } else {
-        const uint32_t a = (y & 0x80008000u) | ((y >> 4) & 0x07F007F0u);
-        const uint32_t b = 0x7B807B80u;
-        r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-    }
+// int8 codes as fp16, exactly: the byte with its sign bit turned, u = code + 128,
+// under the exponent of 1024 is 1024 + u; less 1152 it is the code.
+__device__ __forceinline__ uint32_t int8_half2(uint32_t x) {
+    const uint32_t c = 0x64806480u;
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&c));
     return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t e4m3_half2(uint32_t x) {
+    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)x, __NV_E4M3);
+    return (uint32_t)r.x | (uint32_t)r.y << 16;
+}
+
+// Four codes of a word as two fp16 pairs.
+template <int KIND>
+__device__ __forceinline__ void codes_of_word(uint32_t x, uint32_t& lo, uint32_t& hi) {
+    if (KIND == CHM_INT8) {
+        x ^= 0x80808080u;
+        lo = int8_half2(__byte_perm(x, 0x64646464u, 0x4140));
+        hi = int8_half2(__byte_perm(x, 0x64646464u, 0x4342));
+    } else {
+        lo = e4m3_half2(x & 0xFFFFu);
+        hi = e4m3_half2(x >> 16);
+    }
+}
+
+// Byte e of two words as an fp16 pair.
+template <int KIND>
+__device__ __forceinline__ uint32_t codes_of_pair(uint32_t x, uint32_t y, int e) {
+    if (KIND == CHM_INT8) return int8_half2((__byte_perm(x, y, (uint32_t)(e | (4 + e) << 8)) & 0x00FF00FFu) ^ 0x64806480u);
+    return e4m3_half2(__byte_perm(x, y, (uint32_t)(e | (4 + e) << 4)) & 0xFFFFu);
 }
 
 // ---- how the work is split ------------------------------------------------------
 //
 // A segment is one sequence's tokens for one block of query heads that share a
-// key head.  It is cut into tiles (a step of all warps), and the tiles of all
-// segments, in the order (sequence, block, tile), are dealt out evenly: with
-// `per` = ceil(units / blocks), block c takes units [c * per, (c + 1) * per).
-// So the lengths, which only the device knows, do not matter to the balance, a
-// long sequence spreads over the device and short ones stay whole.  A segment
-// that crosses a block boundary leaves a part (unnormalised output, maximum,
-// sum) per block in the workspace, and attention_join_kernel adds them in order.
-struct Plan {
-    int per;    // units per block
-    int total;  // units
-};
-struct Boundary {  // the first segment of a block
-    int seq, seg;
-    int first, units;  // its first unit, its units
-};
+// key head.  It is cut into units of a tile (a step of all warps), and the units
+// of all segments, in the order (sequence, block, unit), are dealt out evenly:
+// with `per` = ceil(units / blocks), block c takes [c * per, (c + 1) * per).  So
+// the lengths, which only the device knows, do not matter to the balance, a long
+// sequence spreads over the device and short ones stay whole.  A segment that
+// crosses from one block to the next leaves a part (unnormalised output,
+// reference exponent, sum) per block in the workspace, and attention_join_kernel
+// adds them in order.
 
 struct Range {
     int first, end;  // positions attended to
@@ -166,9 +198,8 @@ __device__ __forceinline__ Range sequence_range(const AttArgs& a, int b) {
     return r;
 }
 
-// The parts of a segment of 8 * NT heads: `slots` of [heads][DMAX + 2] floats,
-// the last two the maximum and the sum.  Block c uses slot 2c for the segment
-// that holds its first unit and 2c + 1 for its last.
+// Rows of parts: DMAX output elements, then the reference and the sum.  Block c
+// has slot 2c for the segment that holds its first unit and 2c + 1 for its last.
 template <int DMAX>
 __device__ __forceinline__ float* part_row(float* parts, int slot, int heads, int hh) {
     return parts + ((int64_t)slot * heads + hh) * (DMAX + 4);
@@ -197,9 +228,9 @@ struct Shape {
     // the shared memory that the resident blocks have, about 190 KB per SM.
     static constexpr int kSlot = kTok * DMAX * kBytes;
     static constexpr int kStages = (kResident == 3 ? 8192 : kResident == 2 ? 12288 : 16384) / kSlot;
-    // shared memory: q as operand registers (high and low part), rings, scales;
-    // at a segment's end the warps' parts take the place of the rings
-    static constexpr int kQ = 2 * NT * (DMAX / 32) * 512;
+    // shared memory: q as operand registers, factors of its rows, rings, scales; at a
+    // segment's end the warps' parts take the place of the rings
+    static constexpr int kQ = NT * (DMAX / 32) * 512 + kHeads * 4;
     static constexpr int kRing = kAttWarps * kStages * 2 * kSlot;
     static constexpr int kScales = kWide ? 0 : kAttWarps * kStages * 2 * kTok * 4;
     static constexpr int kRow = DMAX + 4;
@@ -214,31 +245,49 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
     paged_attention_kernel(const AttArgs a) {
     using S = Shape<DMAX, KIND, NT>;
     constexpr bool kWide = S::kWide;
-    constexpr bool kHalf = KIND == CHM_FP16;  // type of the products
+    constexpr bool kHalf = KIND != CHM_BF16;  // fp16 products; 8-bit codes are fp16 numbers
     constexpr int kBytes = S::kBytes, kU = S::kU, kTok = S::kTok, kTile = S::kTile, kHeads = S::kHeads;
     constexpr int kStages = S::kStages, kSlot = S::kSlot;
-    constexpr int kKC = DMAX * kBytes / 64;     // 16-byte runs of a key per thread
-    constexpr int kRuns = DMAX / 32;            // operand runs of q
-    constexpr int kE = DMAX / 8;                // value elements per thread and token
+    constexpr int kKC = DMAX * kBytes / 64;         // 16-byte runs of a key per thread
+    constexpr int kRuns = DMAX / 32;                // operand runs of q
+    constexpr int kE = DMAX / 8;                    // value elements per thread and token
     constexpr int kVB = kE * kBytes < 16 ? 8 : 16;  // bytes of a run of a value
-    constexpr int kVC = kE * kBytes / kVB;      // runs of a value per thread
-    constexpr int kM = kE / 2;                  // 16-row blocks of the output
+    constexpr int kVC = kE * kBytes / kVB;          // runs of a value per thread
+    constexpr int kVT = kVB == 16 ? 4 : 8;          // tokens per copy of values
+    constexpr int kM = kE / 2;                      // 16-row blocks of the output
     constexpr int kRow = S::kRow;
-    static_assert(S::kResident >= 1 && kStages >= 1, "shape");
+    // Weights are exp2(score - ref), where ref trails the largest exponent (score, plus the
+    // log2 of the value's scale) by kLead and moves only when one passes it by kRoom.  fp16
+    // weights (their high part) so stay below 2^15, and the smallest step of their low part,
+    // 2^-24, is 2^-35 of the largest: many small ones are not lost.  bf16 has fp32's range.
+    constexpr float kLead = kHalf ? 11.0f : 0.0f, kRoom = kHalf ? 15.0f : 8.0f;
     extern __shared__ __align__(16) uint8_t smem[];
-    uint4(*s_q)[NT][kRuns][32] = reinterpret_cast<uint4(*)[NT][kRuns][32]>(smem);
+    uint4(*s_q)[kRuns][32] = reinterpret_cast<uint4(*)[kRuns][32]>(smem);
+    float* const s_f = reinterpret_cast<float*>(smem + NT * kRuns * 512);
     float(*s_o)[kHeads][kRow] = reinterpret_cast<float(*)[kHeads][kRow]>(smem + S::kQ);
     float(*s_m)[kHeads] = reinterpret_cast<float(*)[kHeads]>(smem + S::kQ + kAttWarps * kHeads * kRow * 4);
     float(*s_l)[kHeads] = s_m + kAttWarps;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int dim = a.c.dim;
-    // This warp's ring: per stage the keys' runs, then the values', each lane's
-    // own 16 bytes in a row of 512, so that a lane reads back what it copied.
+    // This warp's ring: per stage the keys, then the values.  Keys: a lane's own 16 bytes in
+    // a row of 512, so that it reads back what it copied.  Values: eight lanes copy 128
+    // bytes of a token (a row of four tokens, or of eight 64-byte ones, is one copy of 512);
+    // by lane they would go to memory a sector at a time, which halves the bandwidth (3.7
+    // against 6.7 TB/s).  Lane (g, t) then finds its run in line t, 16-byte places turned by
+    // 2t so that neither side has bank conflicts.
     const uint8_t* const ring = smem + S::kQ + warp * (kStages * 2 * kSlot);
     const float* const scales = reinterpret_cast<const float*>(smem + S::kQ + S::kRing) + warp * (kStages * 2 * kTok);
-    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
-    const uint32_t ring_v = (uint32_t)__cvta_generic_to_shared(ring) + lane * kVB;
+    const uint32_t ring_k = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
+    const int vt = kVB == 16 ? lane >> 3 : lane >> 2;  // the token a lane copies, of kVT
+    const int vc = kVB == 16 ? lane & 7 : lane & 3;    // and its 16 bytes of it
+    const uint32_t ring_v = (uint32_t)__cvta_generic_to_shared(ring) + kSlot +
+                            (kVB == 16 ? vt * 8 + (vc ^ (2 * vt)) : (vt >> 1) * 8 + (((vt & 1) * 4 + vc) ^ (vt & 6))) * 16;
+    // where lane (g, t) reads the values of its first and second token of eight
+    const int run_v0 = kVB == 16 ? (t * 8 + (g ^ (2 * t))) * 16 : t * 128 + ((g >> 1) ^ (2 * t)) * 16 + (g & 1) * 8;
+    const int run_v1 = kVB == 16 ? run_v0 : t * 128 + ((4 + (g >> 1)) ^ (2 * t)) * 16 + (g & 1) * 8;
     const uint32_t scales_at = (uint32_t)__cvta_generic_to_shared(scales) + lane * 4;
+    const char* const kbase = static_cast<const char*>(a.c.k) + t * 16;
+    const char* const vbase = static_cast<const char*>(a.c.v) + vc * 16;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     // ---- this block's units (every warp works them out for itself)
@@ -272,9 +321,6 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
         before += __shfl_sync(0xffffffffu, sum, 31);
     }
     Range r = sequence_range(a, b);
-    const bool split_q = !kWide && a.q_type == CHM_FP16;
-    const char* const kbase = static_cast<const char*>(a.c.k);
-    const char* const vbase = static_cast<const char*>(a.c.v);
 
     for (int piece = 0; u < u1; ++piece) {
         const int in_seq = u - before;
@@ -282,7 +328,10 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
         const int unit0 = in_seq - seg * r.units;
         const int unit1 = min(r.units, unit0 + (u1 - u));
         const bool whole = unit1 - unit0 == r.units;
-        if (piece == 0 && threadIdx.x == 0) a.boundaries[blockIdx.x] = Boundary{b, seg, u - unit0, r.units};
+        if (threadIdx.x == 0) {
+            if (piece == 0) a.boundaries[blockIdx.x] = Boundary{b, seg, u - unit0, r.units};
+            if (in_seq == 0) a.before[b] = before;
+        }
         const int head = seg / a.blocks;
         const int h0 = head * a.group + (seg - head * a.blocks) * kHeads;  // first query head
         const int nh = min(kHeads, (head + 1) * a.group - h0);
@@ -293,56 +342,75 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
 
         // Token `pos` of the range, one per lane: its page, then its place and scales.
         auto page_of = [&](int pos) { return pos < end ? table[a.by_page.div((uint32_t)pos)] : 0; };
-        int64_t at = -1;  // element offset of this lane's token of the newest step, -1: none
+        uint32_t at = kNowhere;  // of this lane's token of the newest step, in 16 bytes
+        bool full = false;       // all the step's tokens are there, in their whole width
         auto place = [&](int pos, int page, int stage) {
-            at = -1;
-            int64_t scale = -1;
+            at = kNowhere;
+            int64_t scale = 0;
             if (pos < end) {
                 if (page < 0 || page >= a.c.num_pages) {
                     bad = true;
                 } else {
                     const uint32_t within = (uint32_t)pos - a.by_page.div((uint32_t)pos) * (uint32_t)a.c.page_size;
-                    at = page * a.c.page_stride + (int64_t)head * a.c.head_stride +
-                         (int64_t)within * a.c.token_stride;
+                    at = (uint32_t)page * a.page16 + (uint32_t)head * a.head16 + within * a.token16;
                     if (!kWide) scale = ((int64_t)page * a.c.heads + head) * a.c.page_size + within;
                 }
             }
             if (!kWide && lane < kTok) {
-                const int64_t x = max(scale, (int64_t)0);
-                copy_async<4>(scales_at + stage * (2 * kTok * 4), a.c.k_scale + x, scale >= 0);
-                copy_async<4>(scales_at + stage * (2 * kTok * 4) + kTok * 4, a.c.v_scale + x, scale >= 0);
+                copy_async_if<4>(scales_at + stage * (2 * kTok * 4), a.c.k_scale + scale, at != kNowhere);
+                copy_async_if<4>(scales_at + stage * (2 * kTok * 4) + kTok * 4, a.c.v_scale + scale, at != kNowhere);
             }
+            full = __all_sync(0xffffffffu, at != kNowhere) && dim == DMAX;
         };
         auto copy_keys = [&](int stage) {
-            const uint32_t to = ring_at + stage * 2 * kSlot;
+            const uint32_t to = ring_k + stage * 2 * kSlot;
 #pragma unroll
-            for (int i = 0; i < kU; ++i)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int64_t x = __shfl_sync(0xffffffffu, at, i * 16 + h * 8 + g);
-                    const char* p = kbase + max(x, (int64_t)0) * kBytes + t * 16;
+            for (int i = 0; i < 2 * kU; ++i) {
+                const uint32_t x = __shfl_sync(0xffffffffu, at, i * 8 + g);
+                const char* p = kbase + (uint64_t)x * 16;
+                if (full) {
+                    copy_async<16, 0>(to + i * kKC * 512, p);
+                    if (kKC > 1) copy_async<16, 64>(to + (i * kKC + 1) * 512, p);
+                    if (kKC > 2) copy_async<16, 128>(to + (i * kKC + 2) * 512, p);
+                    if (kKC > 3) copy_async<16, 192>(to + (i * kKC + 3) * 512, p);
+                    if (kKC > 4) {
+                        copy_async<16, 256>(to + (i * kKC + 4) * 512, p);
+                        copy_async<16, 320>(to + (i * kKC + 5) * 512, p);
+                        copy_async<16, 384>(to + (i * kKC + 6) * 512, p);
+                        copy_async<16, 448>(to + (i * kKC + 7) * 512, p);
+                    }
+                } else {
 #pragma unroll
                     for (int c = 0; c < kKC; ++c) {
-                        const bool in = c * 64 + t * 16 < dim * kBytes;
-                        copy_async<16>(to + ((i * 2 + h) * kKC + c) * 512, in ? p + c * 64 : p, x >= 0 && in);
+                        const bool on = x != kNowhere && c * 64 + t * 16 < dim * kBytes;
+                        copy_async_if<16>(to + (i * kKC + c) * 512, on ? p + c * 64 : kbase, on);
                     }
                 }
+            }
         };
         auto copy_values = [&](int stage) {
-            const uint32_t to = ring_v + stage * 2 * kSlot + kSlot;
+            const uint32_t to = ring_v + stage * 2 * kSlot;
 #pragma unroll
-            for (int i = 0; i < kU; ++i)
-#pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    const int64_t x = __shfl_sync(0xffffffffu, at, i * 16 + (h >> 1) * 8 + 2 * t + (h & 1));
-                    const char* p = vbase + max(x, (int64_t)0) * kBytes;
+            for (int i = 0; i < kTok / kVT; ++i) {
+                // 128-byte runs: tokens 2t or 2t + 1 of eight, as lanes t need them together
+                const int src = kVB == 16 ? (i >> 1) * 8 + 2 * vt + (i & 1) : i * 8 + vt;
+                const uint32_t x = __shfl_sync(0xffffffffu, at, src);
+                const char* p = vbase + (uint64_t)x * 16;
+                if (full) {
+                    copy_async<16, 0>(to + i * kVC * 512, p);
+                    if (kVC > 1) copy_async<16, 128>(to + (i * kVC + 1) * 512, p);
+                    if (kVC > 2) {
+                        copy_async<16, 256>(to + (i * kVC + 2) * 512, p);
+                        copy_async<16, 384>(to + (i * kVC + 3) * 512, p);
+                    }
+                } else {
 #pragma unroll
                     for (int c = 0; c < kVC; ++c) {
-                        const int off = c * 128 + g * kVB;
-                        const bool in = off < dim * kBytes;
-                        copy_async<kVB>(to + ((i * 4 + h) * kVC + c) * (32 * kVB), in ? p + off : p, x >= 0 && in);
+                        const bool on = x != kNowhere && c * 128 + vc * 16 < dim * kBytes;
+                        copy_async_if<16>(to + (i * kVC + c) * 512, on ? p + c * 128 : vbase, on);
                     }
                 }
+            }
         };
 
         int pos = first + warp * kTok + lane % kTok;  // this lane's token of the newest step
@@ -365,36 +433,65 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
             pos += kTile;
         }
 
-        // q: lane (g, t) of a run holds the 8 elements that its key runs meet
-        for (int i = threadIdx.x; i < NT * kRuns * 32; i += kAttThreads) {
-            const int ln = i & 31, run = (i >> 5) % kRuns, nt = (i >> 5) / kRuns;
-            const int hh = nt * 8 + (ln >> 2);
-            const int d0 = kWide ? run * 32 + (ln & 3) * 8 : (run >> 1) * 64 + (ln & 3) * 16 + (run & 1) * 8;
-            uint32_t hi[4], lo[4];
+        // q: lane (g, t) of a run holds the 8 elements that its key runs meet.  For an 8-bit
+        // cache a row is brought by a power of two to a largest element below 2^14, so that
+        // fp16 holds it (exactly but for elements below 2^-28 of the largest).
+        {
+            constexpr int kLanes = DMAX / 8;  // lanes per row
+            const int d0 = (lane % kLanes) * 8;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float x[2];
+            for (int h = 0; h < kHeads; h += kAttWarps * (32 / kLanes)) {
+                const int hh = h + warp * (32 / kLanes) + lane / kLanes;
+                float x[8] = {};
+                const int64_t qa = b * a.q_b + (h0 + hh) * a.q_h + d0;
+                if (hh < nh && d0 < dim) {
+                    uint32_t w[4];
+                    if (a.q_wide) {
+                        const uint4 y = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + qa);
+                        w[0] = y.x, w[1] = y.y, w[2] = y.z, w[3] = y.w;
+                    } else {
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int d = d0 + 2 * j + e;
-                    x[e] = 0.0f;
-                    if (hh < nh && d < dim) {
-                        const int64_t qa = b * a.q_b + (h0 + hh) * a.q_h + d;
-                        x[e] = a.q_type == CHM_FP16 ? __half2float(static_cast<const __half*>(a.q)[qa])
-                                                    : __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[qa]);
+                        for (int e = 0; e < 4; ++e)
+                            w[e] = static_cast<const uint16_t*>(a.q)[qa + 2 * e] |
+                                   (uint32_t) static_cast<const uint16_t*>(a.q)[qa + 2 * e + 1] << 16;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 y = a.q_type == CHM_FP16 ? unpack16<true>(w[e]) : unpack16<false>(w[e]);
+                        x[2 * e] = y.x, x[2 * e + 1] = y.y;
                     }
                 }
-                hi[j] = pack16<kHalf>(x[0], x[1]);
-                const float2 y = unpack16<kHalf>(hi[j]);
-                lo[j] = pack16<kHalf>(x[0] - y.x, x[1] - y.y);
+                float up = 1.0f, f = a.scale_log2;
+                if (!kWide) {
+                    float top = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top = isfinite(x[e]) ? fmaxf(top, fabsf(x[e])) : top;
+#pragma unroll
+                    for (int y = kLanes / 2; y > 0; y >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, y));
+                    const int e = top > 0.0f ? min(13 - ilogbf(top), 100) : 0;
+                    up = exp2f((float)e);
+                    f *= exp2f((float)-e);
+                }
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = pack16<kHalf>(x[2 * e] * up, x[2 * e + 1] * up);
+                const int run = kWide ? d0 / 32 : d0 / 64 * 2 + (d0 / 8) % 2;
+                const int tt = kWide ? d0 / 8 % 4 : d0 / 16 % 4;
+                if (hh < kHeads) {
+                    s_q[hh / 8][run][hh % 8 * 4 + tt] = make_uint4(w[0], w[1], w[2], w[3]);
+                    if (d0 == 0) s_f[hh] = f;
+                }
             }
-            s_q[0][nt][run][ln] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            s_q[1][nt][run][ln] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
         __syncthreads();
+        float qf[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) qf[n][e] = kWide ? a.scale_log2 : s_f[n * 8 + 2 * t + e];
 
         float o[NT][kM][4] = {};
-        float m[NT][2], l[NT][2];
+        float m[NT][2], l[NT][2];  // references and sums of this lane's columns
 #pragma unroll
         for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.0f;
 
@@ -403,7 +500,7 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
         int stage = 0;
         for (; base < end; base += kTile) {
             const uint8_t* const keys = ring + stage * 2 * kSlot + lane * 16;
-            const uint8_t* const values = ring + stage * 2 * kSlot + kSlot + lane * kVB;
+            const uint8_t* const values = ring + stage * 2 * kSlot + kSlot;
             const bool more = base + kStages * kTile < end;
             const int page = next_page;
             next_page = page_of(pos + kTile);
@@ -424,78 +521,93 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
                         uint32_t p0[4], p1[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            if (kWide) {
+                            if (kWide)
                                 p0[e] = w0[e], p1[e] = w1[e];
-                            } else {
-                                const uint32_t x0 = w0[j * 2 + (e >> 1)], x1 = w1[j * 2 + (e >> 1)];
-                                const uint32_t sel =
-                                    KIND == CHM_INT8 ? ((e & 1) ? 0x4342 : 0x4140) : ((e & 1) ? 0x3424 : 0x1404);
-                                p0[e] = codes_to_bf16<KIND>(__byte_perm(x0, 0, sel));
-                                p1[e] = codes_to_bf16<KIND>(__byte_perm(x1, 0, sel));
+                            else if (e % 2 == 0) {
+                                codes_of_word<KIND>(w0[j * 2 + e / 2], p0[e], p0[e + 1]);
+                                codes_of_word<KIND>(w1[j * 2 + e / 2], p1[e], p1[e + 1]);
                             }
                         }
                         const int run = kWide ? c : c * 2 + j;
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            uint4 bq = s_q[0][n][run][lane];
+                            const uint4 bq = s_q[n][run][lane];
                             mma<kHalf>(sc[n][i], p0[0], p1[0], p0[1], p1[1], bq.x, bq.y);
                             mma<kHalf>(sc[n][i], p0[2], p1[2], p0[3], p1[3], bq.z, bq.w);
-                            if (!kWide && split_q) {
-                                bq = s_q[1][n][run][lane];
-                                mma<kHalf>(sc[n][i], p0[0], p1[0], p0[1], p1[1], bq.x, bq.y);
-                                mma<kHalf>(sc[n][i], p0[2], p1[2], p0[3], p1[3], bq.z, bq.w);
-                            }
                         }
                     }
                 }
-            // ---- running maximum; it follows the scores only when one passes it by more than 2^8
-            float vscale[kU][2];
+            // ---- scaled; tokens past the end get weight zero
+            float vs[kU][2], lv[kU][2];
+            if (!kWide) {
+#pragma unroll
+                for (int i = 0; i < kU; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int src = i * 16 + h * 8 + g;
+                        const float ks = scales[stage * 2 * kTok + src];
+                        vs[i][h] = scales[stage * 2 * kTok + kTok + src];
+                        lv[i][h] = fmaxf(log2_fast(fabsf(vs[i][h])), -105.0f);  // the smallest scale written
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) sc[n][i][h * 2 + e] *= ks;
+                    }
+                __syncwarp();  // the scales are read; the next step's take their place
+            }
             bool above = false;
 #pragma unroll
             for (int i = 0; i < kU; ++i)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int src = i * 16 + h * 8 + g;
-                    const bool on = base + src < end;
-                    float f = a.scale_log2;
-                    if (!kWide) {
-                        f *= scales[stage * 2 * kTok + src];
-                        vscale[i][h] = scales[stage * 2 * kTok + kTok + src];
-                    }
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
+                    for (int e = 0; e < 4; ++e) sc[n][i][e] *= qf[n][e & 1];
+            if (base + kTok > end) {
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            float& x = sc[n][i][h * 2 + e];
-                            x = on ? x * f : -INFINITY;
-                            above = above || x > m[n][e] + 8.0f;
+                for (int i = 0; i < kU; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        if (base + i * 16 + h * 8 + g >= end) {
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) sc[n][i][h * 2] = sc[n][i][h * 2 + 1] = -INFINITY;
                         }
-                }
-            if (!kWide) __syncwarp();  // the scales are read; the next step's take their place
+            }
+#pragma unroll
+            for (int i = 0; i < kU; ++i)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        above = above || (kWide ? sc[n][i][e] : sc[n][i][e] + lv[i][e >> 1]) > m[n][e & 1] + kRoom;
             if (more) {
                 place(pos, page, stage);
                 copy_keys(stage);
             }
             copies_commit();
             pos += kTile;
+            // ---- the reference follows the largest exponent
             if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float top = m[n][e];
+                        float top = m[n][e] + kLead;
 #pragma unroll
-                        for (int i = 0; i < kU; ++i) top = fmaxf(top, fmaxf(sc[n][i][e], sc[n][i][2 + e]));
+                        for (int i = 0; i < kU; ++i)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+                                top = fmaxf(top, kWide ? sc[n][i][h * 2 + e] : sc[n][i][h * 2 + e] + lv[i][h]);
 #pragma unroll
                         for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-                        const float f = top == m[n][e] ? 1.0f : exp2_fast(m[n][e] - top);
-                        m[n][e] = top;
+                        top -= kLead;
+                        const float f = top > m[n][e] ? exp2_fast(m[n][e] - top) : 1.0f;
+                        m[n][e] = fmaxf(top, m[n][e]);
                         l[n][e] *= f;
 #pragma unroll
                         for (int i = 0; i < kM; ++i) o[n][i][e] *= f, o[n][i][2 + e] *= f;
                     }
             }
-            // ---- probabilities as the operand of the second product
+            // ---- weights as the operand of the second product, in two 16-bit terms
             uint32_t ph[NT][kU][2], pl[NT][kU][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -506,7 +618,7 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
                     for (int h = 0; h < 2; ++h) {
                         float p0 = exp2_fast(sc[n][i][h * 2] - m0), p1 = exp2_fast(sc[n][i][h * 2 + 1] - m1);
                         l[n][0] += p0, l[n][1] += p1;
-                        if (!kWide) p0 *= vscale[i][h], p1 *= vscale[i][h];
+                        if (!kWide) p0 *= vs[i][h], p1 *= vs[i][h];
                         const uint32_t hi = pack16<kHalf>(p0, p1);
                         const float2 y = unpack16<kHalf>(hi);
                         ph[n][i][h] = transpose8(hi);
@@ -515,6 +627,7 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
             }
             // ---- values
             copies_wait<2 * kStages - 1>();
+            __syncwarp();
 #pragma unroll
             for (int i = 0; i < kU; ++i) {
                 uint32_t vr[4][kVC * kVB / 4];
@@ -522,12 +635,12 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
                 for (int h = 0; h < 4; ++h)
 #pragma unroll
                     for (int c = 0; c < kVC; ++c) {
-                        const uint8_t* x = values + ((i * 4 + h) * kVC + c) * (32 * kVB);
                         if (kVB == 16) {
-                            const uint4 w = *reinterpret_cast<const uint4*>(x);
+                            const uint4 w = *reinterpret_cast<const uint4*>(values + ((i * 4 + h) * kVC + c) * 512 + run_v0);
                             vr[h][c * 4] = w.x, vr[h][c * 4 + 1] = w.y, vr[h][c * 4 + 2] = w.z, vr[h][c * 4 + 3] = w.w;
                         } else {
-                            const uint2 w = *reinterpret_cast<const uint2*>(x);
+                            const uint2 w = *reinterpret_cast<const uint2*>(values + (i * 2 + (h >> 1)) * 512 +
+                                                                            (h & 1 ? run_v1 : run_v0));
                             vr[h][0] = w.x, vr[h][1] = w.y;
                         }
                     }
@@ -539,15 +652,10 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
                         const int x = j + (h & 1) * kM;
                         const uint32_t* v0 = vr[(h >> 1) * 2];
                         const uint32_t* v1 = vr[(h >> 1) * 2 + 1];
-                        if (kWide) {
+                        if (kWide)
                             f[h] = __byte_perm(v0[x / 2], v1[x / 2], (x & 1) ? 0x7632 : 0x5410);
-                        } else {
-                            // the codes in the low (int8) or high (e4m3) bytes of the halves
-                            const int e = x & 3;
-                            const uint32_t sel =
-                                KIND == CHM_INT8 ? (uint32_t)(e | (4 + e) << 8) : (uint32_t)(e << 4 | (4 + e) << 12);
-                            f[h] = codes_to_bf16<KIND>(__byte_perm(v0[x / 4], v1[x / 4], sel));
-                        }
+                        else
+                            f[h] = codes_of_pair<KIND>(v0[x / 4], v1[x / 4], x & 3);
                     }
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
@@ -556,7 +664,10 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
                     }
                 }
             }
-            if (more) copy_values(stage);
+            if (more) {
+                __syncwarp();  // all lanes have read these slots
+                copy_values(stage);
+            }
             copies_commit();
             stage = stage + 1 == kStages ? 0 : stage + 1;
         }
@@ -619,61 +730,76 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
     }
 }
 
-// Block (c, h): if the first segment of block c + 1 began in block c, head h of
-// that segment from its parts, in the order of the blocks.
-constexpr int kJoinThreads = 128;
+// Block (x, h): head h of a segment that several blocks had, from its parts in
+// the order of the blocks.  x stands for a segment or, where there are fewer, for
+// the boundary before block x + 1 (then the segment's first boundary does it).
+constexpr int kJoinThreads = 256;
 
 template <int DMAX, int NT>
 __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const AttArgs a) {
     constexpr int kHeads = 8 * NT;
-    constexpr int kWarps = kJoinThreads / 32;
-    constexpr int kV = DMAX / 32;  // elements per lane
-    __shared__ float s_acc[kWarps][DMAX];
-    __shared__ float s_top[kWarps], s_sum[kWarps];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int kV = DMAX / 32;   // elements per lane
+    constexpr int kAhead = kV > 4 ? 4 : 8;  // parts on their way per warp
+    __shared__ float s_acc[kJoinThreads / 32][DMAX];
+    __shared__ float s_sum[kJoinThreads / 32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int per = a.plan->per;
-    const int c = blockIdx.x + 1;
-    if (c * (int64_t)per >= a.plan->total) return;
-    const Boundary s = a.boundaries[c];
-    const int c0 = s.first / per, c1 = (s.first + s.units - 1) / per;
-    if (s.first == c * per || c != c0 + 1) return;
+    const Plan plan = *a.plan;
+    const int segs = a.c.heads * a.blocks;
+    Boundary s;
+    if (a.join_segments) {
+        s.seq = blockIdx.x / segs;
+        s.seg = blockIdx.x - s.seq * segs;
+        s.units = sequence_range(a, s.seq).units;
+        s.first = a.before[s.seq] + s.seg * s.units;
+    } else {
+        const int64_t u = (blockIdx.x + 1) * (int64_t)plan.per;
+        if (u >= plan.total) return;
+        s = a.boundaries[blockIdx.x + 1];
+        if (s.first == u || s.first / plan.per != (int)blockIdx.x) return;
+    }
+    const int c0 = s.first / plan.per, c1 = (s.first + s.units - 1) / plan.per;
+    if (c0 == c1) return;
     const int head = s.seg / a.blocks;
     const int h0 = head * a.group + (s.seg - head * a.blocks) * kHeads;
     const int hh = blockIdx.y;
     if (h0 + hh >= (head + 1) * a.group) return;
-    // each warp: every kWarps-th part, with a running maximum
-    float top = -INFINITY, sum = 0.0f, acc[kV] = {};
-#pragma unroll 4
-    for (int i = c0 + warp; i <= c1; i += kWarps) {
-        const int slot = 2 * i + (i == c0 && c0 * per != s.first);
-        const float* part = part_row<DMAX>(a.parts, slot, kHeads, hh);
-        const float m = part[DMAX], l = part[DMAX + 1];
-        const float now = fmaxf(top, m);
-        const float f = top == now ? 1.0f : exp2_fast(top - now);
-        const float w = m == -INFINITY ? 0.0f : exp2_fast(m - now);
-        top = now;
-        sum = sum * f + l * w;
+    const int odd = c0 * plan.per != s.first;  // whether the first part is its block's second slot
+    auto part = [&](int i) { return part_row<DMAX>(a.parts, 2 * i + (i == c0 ? odd : 0), kHeads, hh); };
+    // each warp takes every warps-th part; the largest reference first, then the sums
+    float top = -INFINITY;
+    for (int i = c0 + lane; i <= c1; i += 32) top = fmaxf(top, part(i)[DMAX]);
 #pragma unroll
-        for (int v = 0; v < kV; ++v) acc[v] = acc[v] * f + part[v * 32 + lane] * w;
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    float sum = 0.0f, acc[kV] = {};
+    for (int i = c0 + warp; i <= c1; i += warps * kAhead) {
+        float x[kAhead][kV], w[kAhead], l[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const bool on = i + j * warps <= c1;
+            const float* p = part(on ? i + j * warps : i);
+            const float m = p[DMAX];
+            w[j] = on && m != -INFINITY ? exp2_fast(m - top) : 0.0f;
+            l[j] = on ? p[DMAX + 1] : 0.0f;
+#pragma unroll
+            for (int v = 0; v < kV; ++v) x[j][v] = on ? p[v * 32 + lane] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            sum += l[j] * w[j];
+#pragma unroll
+            for (int v = 0; v < kV; ++v) acc[v] += x[j][v] * w[j];
+        }
     }
 #pragma unroll
     for (int v = 0; v < kV; ++v) s_acc[warp][v * 32 + lane] = acc[v];
-    if (lane == 0) s_top[warp] = top, s_sum[warp] = sum;
+    if (lane == 0) s_sum[warp] = sum;
     __syncthreads();
-    top = -INFINITY, sum = 0.0f;
-    float f[kWarps];
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_top[w]);
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        f[w] = s_top[w] == -INFINITY ? 0.0f : exp2_fast(s_top[w] - top);
-        sum += f[w] * s_sum[w];
-    }
-    for (int d = threadIdx.x; d < a.c.dim; d += kJoinThreads) {
+    sum = 0.0f;
+    for (int w = 0; w < warps; ++w) sum += s_sum[w];
+    for (int d = threadIdx.x; d < a.c.dim; d += blockDim.x) {
         float y = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) y += f[w] * s_acc[w][d];
+        for (int w = 0; w < warps; ++w) y += s_acc[w][d];
         store_row(a, s.seq, h0 + hh, d, sum == 0.0f ? 0.0f : sum != sum ? sum : y / sum);
     }
     if (threadIdx.x == 0 && a.lse)
@@ -695,9 +821,19 @@ static int sm_count() {
     return cached[dev] = n;
 }
 
+// Runs of units per resident block.  The SMs do not run alike (64 sequences up to
+// 4,096 tokens, one run each: the busiest SM is busy for 1.25 times the mean), so
+// later runs go to the blocks that are done first.
+#ifndef CHM_WAVES
+#define CHM_WAVES 1
+#endif
+constexpr int kWaves = CHM_WAVES;
+
 struct Layout {
     int blocks;       // thread blocks of the main kernel
+    int segs;         // segments per sequence
     int unit_tokens;  // tokens per unit
+    int64_t units;    // at most
     bool joins;       // whether a segment can be split
 };
 
@@ -711,33 +847,10 @@ struct Launch {
         const int whole = 4 * S::kTile;
         y.unit_tokens = a.capacity <= whole ? whole : S::kTile;
         y.joins = a.capacity > whole;
-        const int64_t segs = (int64_t)a.c.heads * ((a.group + S::kHeads - 1) / S::kHeads);
-        const int64_t units = a.batch * segs * std::max<int64_t>(1, ((int64_t)a.capacity + y.unit_tokens - 1) / y.unit_tokens);
-        y.blocks = (int)std::min<int64_t>(units, (int64_t)sm_count() * S::kResident);
+        y.segs = a.c.heads * ((a.group + S::kHeads - 1) / S::kHeads);
+        y.units = (int64_t)a.batch * y.segs * std::max(1, (a.capacity + y.unit_tokens - 1) / y.unit_tokens);
+        y.blocks = (int)std::min<int64_t>(y.units, (int64_t)sm_count() * S::kResident * kWaves);
         return y;
-    }
-    // Units are counted in 32 bits.
-    static bool fits(const AttArgs& a) {
-        const Layout y = layout(a);
-        const int64_t segs = (int64_t)a.c.heads * ((a.group + S::kHeads - 1) / S::kHeads);
-        const int64_t per_seq = std::max<int64_t>(1, ((int64_t)a.capacity + y.unit_tokens - 1) / y.unit_tokens);
-        return segs * per_seq <= (INT32_MAX - (1 << 16)) / std::max(1, a.batch);
-    }
-    template <typename A>
-    static void carve(A& arena, const Layout& y, AttArgs* a) {
-        auto plan = arena.template take<Plan>(1);
-        auto bounds = arena.template take<Boundary>(y.blocks);
-        auto parts = arena.template take<float>(y.joins ? (size_t)2 * y.blocks * S::kHeads * (DMAX + 4) : 0);
-        if (a) {
-            a->plan = (Plan*)plan;
-            a->boundaries = (Boundary*)bounds;
-            a->parts = (float*)parts;
-        }
-    }
-    static size_t workspace(const AttArgs& a) {
-        Counter c;
-        carve(c, layout(a), nullptr);
-        return c.s.off;
     }
     struct Counter {
         Sizer s;
@@ -747,14 +860,38 @@ struct Launch {
             return nullptr;
         }
     };
+    template <typename A>
+    static void carve(A& arena, const Layout& y, AttArgs* a, int batch) {
+        auto plan = arena.template take<Plan>(1);
+        auto before = arena.template take<int32_t>(batch);
+        auto bounds = arena.template take<Boundary>(y.blocks);
+        auto parts = arena.template take<float>(y.joins ? (size_t)2 * y.blocks * S::kHeads * (DMAX + 4) : 0);
+        if (a) {
+            a->plan = (Plan*)plan;
+            a->before = (int32_t*)before;
+            a->boundaries = (Boundary*)bounds;
+            a->parts = (float*)parts;
+        }
+    }
+    static size_t workspace(const AttArgs& a) {
+        Counter c;
+        carve(c, layout(a), nullptr, a.batch);
+        return c.s.off;
+    }
     static chm_status run(AttArgs a, void* ws, size_t ws_bytes, cudaStream_t st) {
         const Layout y = layout(a);
+        if (y.units > INT32_MAX - (1 << 20)) {  // units are counted in 32 bits
+            set_last_message("paged_attention: too much work for one call");
+            return CHM_ERR_INVALID;
+        }
         Arena arena(ws, ws_bytes);
-        carve(arena, y, &a);
+        carve(arena, y, &a, a.batch);
         if (arena.overflow) return CHM_ERR_CAPACITY;
         a.blocks = (a.group + S::kHeads - 1) / S::kHeads;
         a.unit_tokens = y.unit_tokens;
         a.by_unit = FastDiv((uint32_t)y.unit_tokens);
+        const int64_t segments = (int64_t)a.batch * y.segs;
+        a.join_segments = segments < y.blocks;
         static bool set[64];  // per device: the kernel may take this much shared memory
         int dev = 0;
         CHM_CUDA(cudaGetDevice(&dev));
@@ -766,10 +903,11 @@ struct Launch {
         paged_attention_kernel<DMAX, KIND, NT><<<(unsigned)y.blocks, kAttThreads, S::kShared, st>>>(a);
         CHM_TRY(launch_status("paged_attention_kernel"));
         if (!y.joins || y.blocks < 2) return CHM_OK;
-        // The join's blocks start while the main kernel's last ones run, and wait for its end.
+        // The join's blocks start while the main kernel's last ones run, and wait for its
+        // end.  Few segments have many parts each: more warps to add them.
         cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3((unsigned)(y.blocks - 1), (unsigned)std::min(S::kHeads, a.group));
-        cfg.blockDim = dim3(kJoinThreads);
+        cfg.gridDim = dim3((unsigned)(a.join_segments ? segments : y.blocks - 1), (unsigned)std::min(S::kHeads, a.group));
+        cfg.blockDim = dim3(segments * 32 < y.blocks ? kJoinThreads : 64);
         cfg.stream = st;
         cudaLaunchAttribute attr{};
         attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -799,6 +937,14 @@ static auto with_launch(const AttArgs& a, F f) {
         case CHM_INT8: return with_kind<CHM_INT8>(a, f);
         default: return with_kind<CHM_E4M3>(a, f);
     }
+}
+
+// Whether 32 bits of 16 bytes reach every vector of the cache.
+static bool spans_64gb(const chm_kv_cache& c) {
+    const unsigned __int128 n = (unsigned __int128)(uint64_t)std::max<int64_t>(c.num_pages - 1, 0) * (uint64_t)c.page_stride +
+                                (unsigned __int128)(uint64_t)(c.heads - 1) * (uint64_t)c.head_stride +
+                                (unsigned __int128)(uint64_t)(c.page_size - 1) * (uint64_t)c.token_stride;
+    return n * type_bytes(c.type) / 16 < kNowhere;
 }
 
 static chm_status refuse_attention(const char* why) {
@@ -843,9 +989,15 @@ extern "C" chm_status chm_paged_attention(const chm_kv_cache* cache, const chm_h
     if ((int64_t)table_width * cache->page_size > (1 << 30)) return refuse_attention("a table spans at most 2^30 tokens");
     if (batch == 0) return CHM_OK;
     if (!q->data || !out->data || !lens || (table_width > 0 && !tables)) return refuse_attention("null pointer");
+    if (!spans_64gb(*cache)) return refuse_attention("keys and values span at most 64 GB each");
     AttArgs a{};
     a.c = *cache;
+    const int run = 16 / type_bytes(cache->type);
+    a.page16 = (uint32_t)(cache->page_stride / run);
+    a.head16 = (uint32_t)(cache->head_stride / run);
+    a.token16 = (uint32_t)(cache->token_stride / run);
     a.q = q->data;
+    a.q_wide = aligned16(q->data) && q->batch_stride % 8 == 0 && q->head_stride % 8 == 0;
     a.out = out->data;
     a.q_b = q->batch_stride, a.q_h = q->head_stride, a.out_b = out->batch_stride, a.out_h = out->head_stride;
     a.q_type = type;
@@ -861,6 +1013,5 @@ extern "C" chm_status chm_paged_attention(const chm_kv_cache* cache, const chm_h
     a.lse = lse;
     a.by_page = FastDiv((uint32_t)cache->page_size);
     cudaStream_t st = (cudaStream_t)stream;
-    if (!with_launch(a, [&](auto l) { return l.fits(a); })) return refuse_attention("too much work for one call");
     return with_launch(a, [&](auto l) { return l.run(a, workspace, workspace_bytes, st); });
 }

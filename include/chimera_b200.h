@@ -428,9 +428,7 @@ chm_status chm_cache_write(const chm_kv_cache* cache, const chm_heads* k, const 
                            int64_t tokens, const int64_t* slots, void* stream);
 
 /* Read slots back: k, v [tokens, heads, dim] of `type`, code * scale in fp32
- * rounded to the type.  A slot below 0 or past the last page reads as zeros.
- * (e4m3: the NaN codes 0x7f and 0xff, which chm_cache_write never writes, count
- * as +-480, here and in chm_paged_attention.) */
+ * rounded to the type.  A slot below 0 or past the last page reads as zeros. */
 chm_status chm_cache_read(const chm_kv_cache* cache, const int64_t* slots, int64_t tokens, const chm_heads* k,
                           const chm_heads* v, int32_t type, void* stream);
 
@@ -449,10 +447,13 @@ chm_status chm_cache_read(const chm_kv_cache* cache, const int64_t* slots, int64
  * the range are not read.  A page id outside the cache that the range needs,
  * or a length past the table's end, makes the sequence's rows and lse NaN.
  * Softmax statistics and sums are fp32; probabilities enter the value product
- * as two 16-bit terms (high and remainder).  A sequence may be cut elsewhere in
+ * as two 16-bit terms (high and remainder); beside 8-bit caches q enters the
+ * score product as fp16, brought into its range by a power of two per row
+ * (exact but for elements below 2^-28 of the row's largest).  A sequence may be cut elsewhere in
  * another batch or with a wider table, which moves the rounding of its sums;
  * the same call gives the same bits every time.
- * table_width * page_size is at most 2^30, batch 65,535.  Calls on one
+ * table_width * page_size is at most 2^30, batch 65,535, and the keys' and the
+ * values' memory span at most 64 GB each.  Calls on one
  * workspace must not overlap. */
 size_t chm_paged_attention_workspace_bytes(const chm_kv_cache* cache, int64_t batch, int32_t q_heads,
                                            int32_t table_width);
