@@ -52,6 +52,7 @@ struct AttArgs {
     int64_t table_stride;
     int32_t capacity;     // table_width * page_size
     int32_t unit_tokens;  // tokens per unit of work
+    int32_t start_units;  // units that a segment counts before its tokens
     FastDiv by_unit, by_page;
     const int32_t* lens;
     const int32_t* starts;
@@ -177,10 +178,16 @@ __device__ __forceinline__ uint32_t codes_of_pair(uint32_t x, uint32_t y, int e)
 // of all segments, in the order (sequence, block, unit), are dealt out evenly:
 // with `per` = ceil(units / blocks), block c takes [c * per, (c + 1) * per).  So
 // the lengths, which only the device knows, do not matter to the balance, a long
-// sequence spreads over the device and short ones stay whole.  A segment that
+// sequence spreads over the device and short ones stay whole.  A segment counts
+// kStartUnits more, before its first tile, for what its start and end cost: blocks
+// with many short segments were the last to finish (64 sequences up to 4,096
+// tokens: 110 us with none, 104 / 102 / 101 / 102 with 1 / 2 / 3 / 5; 128 long
+// documents e4m3: 43.5, 39.3 / 39.3 / 39.5 / 41.3).  A segment that
 // crosses from one block to the next leaves a part (unnormalised output,
 // reference exponent, sum) per block in the workspace, and attention_join_kernel
 // adds them in order.
+
+constexpr int kStartUnits = 2;
 
 struct Range {
     int first, end;  // positions attended to
@@ -194,7 +201,7 @@ __device__ __forceinline__ Range sequence_range(const AttArgs& a, int b) {
     r.end = a.lens[b];
     r.bad = r.end > a.capacity;
     if (r.bad) r.end = 0;
-    r.units = max(1, (int)a.by_unit.div((uint32_t)(max(r.end - r.first, 0) + a.unit_tokens - 1)));
+    r.units = a.start_units + max(1, (int)a.by_unit.div((uint32_t)(max(r.end - r.first, 0) + a.unit_tokens - 1)));
     return r;
 }
 
@@ -336,8 +343,8 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
         const int h0 = head * a.group + (seg - head * a.blocks) * kHeads;  // first query head
         const int nh = min(kHeads, (head + 1) * a.group - h0);
         const int32_t* table = a.tables + b * a.table_stride;
-        const int first = r.first + unit0 * a.unit_tokens;
-        const int end = unit1 == r.units ? r.end : r.first + unit1 * a.unit_tokens;
+        const int first = r.first + max(unit0 - a.start_units, 0) * a.unit_tokens;
+        const int end = unit1 == r.units ? r.end : r.first + max(unit1 - a.start_units, 0) * a.unit_tokens;
         bool bad = r.bad;
 
         // Token `pos` of the range, one per lane: its page, then its place and scales.
@@ -821,18 +828,11 @@ static int sm_count() {
     return cached[dev] = n;
 }
 
-// Runs of units per resident block.  The SMs do not run alike (64 sequences up to
-// 4,096 tokens, one run each: the busiest SM is busy for 1.25 times the mean), so
-// later runs go to the blocks that are done first.
-#ifndef CHM_WAVES
-#define CHM_WAVES 1
-#endif
-constexpr int kWaves = CHM_WAVES;
-
 struct Layout {
     int blocks;       // thread blocks of the main kernel
     int segs;         // segments per sequence
     int unit_tokens;  // tokens per unit
+    int start_units;
     int64_t units;    // at most
     bool joins;       // whether a segment can be split
 };
@@ -847,9 +847,10 @@ struct Launch {
         const int whole = 4 * S::kTile;
         y.unit_tokens = a.capacity <= whole ? whole : S::kTile;
         y.joins = a.capacity > whole;
+        y.start_units = y.joins ? kStartUnits : 0;  // else a segment is one unit
         y.segs = a.c.heads * ((a.group + S::kHeads - 1) / S::kHeads);
-        y.units = (int64_t)a.batch * y.segs * std::max(1, (a.capacity + y.unit_tokens - 1) / y.unit_tokens);
-        y.blocks = (int)std::min<int64_t>(y.units, (int64_t)sm_count() * S::kResident * kWaves);
+        y.units = (int64_t)a.batch * y.segs * (y.start_units + std::max(1, (a.capacity + y.unit_tokens - 1) / y.unit_tokens));
+        y.blocks = (int)std::min<int64_t>(y.units, (int64_t)sm_count() * S::kResident);
         return y;
     }
     struct Counter {
@@ -889,6 +890,7 @@ struct Launch {
         if (arena.overflow) return CHM_ERR_CAPACITY;
         a.blocks = (a.group + S::kHeads - 1) / S::kHeads;
         a.unit_tokens = y.unit_tokens;
+        a.start_units = y.start_units;
         a.by_unit = FastDiv((uint32_t)y.unit_tokens);
         const int64_t segments = (int64_t)a.batch * y.segs;
         a.join_segments = segments < y.blocks;
