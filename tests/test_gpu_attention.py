@@ -298,6 +298,31 @@ def test_cache_codes_at_ties_and_neighbours(held):
 
 
 @pytest.mark.parametrize("held", ["int8", "e4m3"])
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+def test_cache_codes_of_every_fraction(t, held):
+    """Every fraction of a 16-bit type under every largest value's fraction, over the exponents that get codes: exact
+    ties, scales rounded up, down and not at all."""
+    ht, dt = NAMES[held], NAMES[t]
+    bits = 8 if t == "bf16" else 11
+    n = 1 << (bits - 1)
+    part = torch.arange(n, 2 * n, device=DEV, dtype=torch.float64) / n    # 1 to 2
+    for e in range(0, 20 if held == "e4m3" else 10):
+        lot = torch.cat([part, torch.zeros(-n % 127, device=DEV, dtype=torch.float64)]).view(-1, 127) * 2.0 ** -e
+        x = torch.zeros(n, lot.shape[0], 128, device=DEV, dtype=torch.float64)
+        x[:, :, :127] = lot
+        x[:, :, 127] = 2.0 if e == 0 else 1.0
+        x[:, :, 127] *= part[:, None]
+        x = x.view(-1, 1, 128)
+        sign = torch.where(torch.arange(128, device=DEV) % 2 == 0, 1.0, -1.0)
+        y = (x * sign).to(dt)
+        kp, vp, ks, vs = make_pages(y.shape[0], 1, 1, 128, ht)
+        A.cache_write(y, y, torch.arange(y.shape[0], device=DEV), kp, vp, ks, vs)
+        code, scale = quantised64(y, ht)
+        assert torch.equal(ks[:, :, 0], scale)
+        assert torch.equal(kp.view(-1, 128).double(), code.view(-1, 128))
+
+
+@pytest.mark.parametrize("held", ["int8", "e4m3"])
 def test_cache_holds_odd_vectors(held):
     ht = NAMES[held]
     x = torch.ones(8, 2, 32, device=DEV)
