@@ -5,7 +5,9 @@
 // the gradient turns back by the same angle.  The angle is reduced to turns in
 // 64 bits (p * f_i / 2 pi less its nearest integer), since 32 bits lose
 // whole turns at far positions; what is left takes 32-bit sine and cosine.
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "vectors.cuh"
 
@@ -26,88 +28,161 @@ struct RotaryArgs {
     int64_t pos_b, pos_t;
     const double* freqs;
     float scale;
-    float sign;  // -1: turn back
-    int64_t rows;
-    int64_t tokens;  // per batch row
-    int32_t chunks;  // items per vector
-    int32_t turn_chunks;
-    FastDiv by_chunks;
+    float sign;            // -1: turn back
+    int32_t rows, tokens;  // tokens in all, and per batch row
+    int32_t parts;         // warps that share a row
+    int32_t chunks, turn_chunks;  // items per vector, and those that turn
+    int32_t lanes;         // lanes across a vector: a power of two
+    FastDiv by_tokens, by_parts;
 };
 
-constexpr int kRotaryThreads = 256;
-
-// Block: one row (a token of a batch row), all heads.  An item is V pairs of a vector: two runs
-// of V elements that one thread loads, turns and stores (so in place is safe).
-template <typename T, int V, bool INTER>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const RotaryArgs a) {
-    extern __shared__ float2 s_turn[];  // (cos, sin) * scale of the row's pairs
-    const int64_t row = blockIdx.x;
-    const int64_t b = row / a.tokens, t = row - b * a.tokens;
-    const int64_t at = b * a.pos_b + t * a.pos_t;
-    const double pos = a.position_bytes == 8 ? (double)static_cast<const int64_t*>(a.positions)[at]
-                                             : (double)static_cast<const int32_t*>(a.positions)[at];
-    for (int i = threadIdx.x; i < a.rot / 2; i += kRotaryThreads) {
-        const double turns = pos * (a.freqs[i] * 0.15915494309189533577);  // 1 / (2 pi)
-        float s, c;
-        sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-        s_turn[i] = make_float2(a.scale * c, a.sign * a.scale * s);
+// V elements of a run, as pairs of floats.
+template <typename T, int V>
+struct Run {
+    Pack<T, V> p;
+    __device__ __forceinline__ void floats(float (&f)[V]) const {
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = to_float<T>(p.v[i]);
     }
-    __syncthreads();
-    const int half = a.rot / 2;
-    const int items = a.heads * a.chunks;
-    for (int it = threadIdx.x; it < items; it += kRotaryThreads) {
-        const int h = (int)a.by_chunks.div((uint32_t)it);
-        const int c = it - h * a.chunks;
-        const bool second = h >= a.heads0;
-        const HeadsView& v = a.set[second];
-        const int hh = second ? h - a.heads0 : h;
-        const T* in = static_cast<const T*>(v.in) + b * v.in_b + t * v.in_t + hh * v.in_h;
-        T* out = static_cast<T*>(v.out) + b * v.out_b + t * v.out_t + hh * v.out_h;
-        using P = Pack<T, V>;
-        if (c < a.turn_chunks) {
-            const int o0 = INTER ? 2 * c * V : c * V;
-            const int o1 = INTER ? o0 + V : half + o0;
-            P x = *reinterpret_cast<const P*>(in + o0), y = *reinterpret_cast<const P*>(in + o1);
-            if (INTER) {
-                // x, y: 2V neighbours, V pairs
-                float e[2 * V];
+    __device__ __forceinline__ void set(const float* f) {
+        if (V > 1 && sizeof(T) == 2) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) e[j] = to_float<T>(x.v[j]), e[V + j] = to_float<T>(y.v[j]);
+            for (int i = 0; i < V; i += 2) two(f[i], f[(i + 1) % V], i);
+        } else {
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float2 w = s_turn[c * V + j];
-                    const float p = e[2 * j], q = e[2 * j + 1];
-                    e[2 * j] = p * w.x - q * w.y;
-                    e[2 * j + 1] = p * w.y + q * w.x;
-                }
+            for (int i = 0; i < V; ++i) p.v[i] = from_float<T>(f[i]);
+        }
+    }
+    __device__ __forceinline__ void two(float a, float b, int i);
+};
+template <typename T, int V>
+__device__ __forceinline__ void Run<T, V>::two(float a, float b, int i) {
+    if constexpr (std::is_same<T, __half>::value)
+        *reinterpret_cast<__half2*>(&p.v[i]) = __floats2half2_rn(a, b);
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        *reinterpret_cast<__nv_bfloat162*>(&p.v[i]) = __floats2bfloat162_rn(a, b);
+}
+
+constexpr int kRotaryAhead = 3;  // vectors' items a lane has on their way, two 16-byte loads each
+
+// A warp (or `parts` of them) has a row: a token's vectors of all heads.  Its lanes stand in
+// rows of a.lanes across a vector, so that a lane keeps its place in the vector and the sine
+// and cosine of its V pairs from head to head.  An item is V pairs: two runs of V elements
+// that one lane loads, turns and stores (so in place is safe).  The first items are loaded
+// before the row's angles are worked out, two or so per lane, into the warp's own table:
+// the V pairs of an item as groups of 16 bytes, each group's items in a row.
+template <typename T, int V, bool INTER>
+__global__ void __launch_bounds__(128, 6) rotary_kernel(const RotaryArgs a) {
+    using R = Run<T, V>;
+    extern __shared__ __align__(16) float2 s_turn[];  // (cos, sin) * scale
+    constexpr int kGroup = V > 1 ? 2 : 1;
+    const int half = a.rot / 2, lane = threadIdx.x & 31;
+    float2* const table = s_turn + (threadIdx.x >> 5) * half;
+    const int warp = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    const int row = (int)a.by_parts.div((uint32_t)warp), part = warp - row * a.parts;
+    if (row >= a.rows) return;
+    const int b = (int)a.by_tokens.div((uint32_t)row), t = row - b * a.tokens;
+    const T* in[2];
+    T* out[2];
 #pragma unroll
-                for (int j = 0; j < V; ++j) x.v[j] = from_float<T>(e[j]), y.v[j] = from_float<T>(e[V + j]);
-            } else {
+    for (int i = 0; i < 2; ++i) {
+        in[i] = static_cast<const T*>(a.set[i].in) + b * a.set[i].in_b + t * a.set[i].in_t;
+        out[i] = static_cast<T*>(a.set[i].out) + b * a.set[i].out_b + t * a.set[i].out_t;
+    }
+    const int per_step = 32 / a.lanes;            // heads a warp has at a time
+    const int step = per_step * a.parts;
+    const int h0 = part * per_step + lane / a.lanes;
+    bool ready = false;
+    for (int c = lane % a.lanes; c - lane % a.lanes < a.chunks; c += a.lanes) {
+        // this lane's runs of a vector
+        const bool turns = c < a.turn_chunks, on = c < a.chunks;
+        const int o0 = turns ? (INTER ? 2 * c * V : c * V) : a.rot + 2 * (c - a.turn_chunks) * V;
+        const int o1 = turns && !INTER ? half + o0 : o0 + V;
+        const bool second = o1 < a.dim;
+        float2 w[V];
+        for (int h = h0; h - lane / a.lanes < a.heads; h += step * kRotaryAhead) {
+            R x[kRotaryAhead], y[kRotaryAhead];
+            T* to[kRotaryAhead];
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float2 w = s_turn[c * V + j];
-                    const float p = to_float<T>(x.v[j]), q = to_float<T>(y.v[j]);
-                    x.v[j] = from_float<T>(p * w.x - q * w.y);
-                    y.v[j] = from_float<T>(p * w.y + q * w.x);
+            for (int u = 0; u < kRotaryAhead; ++u) {
+                const int hu = h + u * step;
+                to[u] = nullptr;
+                if (on && hu < a.heads) {
+                    const bool k = hu >= a.heads0;
+                    const int hh = k ? hu - a.heads0 : hu;
+                    const T* from = (k ? in[1] : in[0]) + hh * (k ? a.set[1].in_h : a.set[0].in_h) + o0;
+                    to[u] = (k ? out[1] : out[0]) + hh * (k ? a.set[1].out_h : a.set[0].out_h) + o0;
+                    if (!turns && from == to[u]) {
+                        to[u] = nullptr;  // passed on in place
+                    } else {
+                        x[u].p = *reinterpret_cast<const Pack<T, V>*>(from);
+                        if (second) y[u].p = *reinterpret_cast<const Pack<T, V>*>(from + (o1 - o0));
+                    }
                 }
             }
-            *reinterpret_cast<P*>(out + o0) = x;
-            *reinterpret_cast<P*>(out + o1) = y;
-        } else if (in != out) {
-            const int o0 = a.rot + 2 * (c - a.turn_chunks) * V;
-            *reinterpret_cast<P*>(out + o0) = *reinterpret_cast<const P*>(in + o0);
-            if (o0 + V < a.dim) *reinterpret_cast<P*>(out + o0 + V) = *reinterpret_cast<const P*>(in + o0 + V);
+            if (!ready) {
+                const int64_t at = b * a.pos_b + t * a.pos_t;
+                const double pos = a.position_bytes == 8 ? (double)static_cast<const int64_t*>(a.positions)[at]
+                                                         : (double)static_cast<const int32_t*>(a.positions)[at];
+                for (int i = lane; i < half; i += 32) {
+                    const double turn = pos * (a.freqs[i] * 0.15915494309189533577);  // 1 / (2 pi)
+                    float sine, cosine;
+                    sincospif(2.0f * (float)(turn - rint(turn)), &sine, &cosine);
+                    const int item = i / V, j = i % V;
+                    table[(j / kGroup * a.turn_chunks + item) * kGroup + j % kGroup] =
+                        make_float2(a.scale * cosine, a.sign * a.scale * sine);
+                }
+                __syncwarp();
+                ready = true;
+            }
+            if (h == h0 && turns) {
+#pragma unroll
+                for (int j = 0; j < V; j += kGroup) {
+                    const float2* p = table + (j / kGroup * a.turn_chunks + c) * kGroup;
+                    if (kGroup == 2) {
+                        const float4 f = *reinterpret_cast<const float4*>(p);
+                        w[j] = make_float2(f.x, f.y), w[(j + 1) % V] = make_float2(f.z, f.w);
+                    } else {
+                        w[j] = *p;
+                    }
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kRotaryAhead; ++u) {
+                if (!to[u]) continue;
+                if (turns) {
+                    float e[2][V];
+                    x[u].floats(e[0]);
+                    y[u].floats(e[1]);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        float &p = INTER ? e[2 * j / V][2 * j % V] : e[0][j];
+                        float &q = INTER ? e[(2 * j + 1) / V][(2 * j + 1) % V] : e[1][j];
+                        const float p0 = p;
+                        p = p0 * w[j].x - q * w[j].y;
+                        q = p0 * w[j].y + q * w[j].x;
+                    }
+                    x[u].set(e[0]);
+                    y[u].set(e[1]);
+                }
+                *reinterpret_cast<Pack<T, V>*>(to[u]) = x[u].p;
+                if (second) *reinterpret_cast<Pack<T, V>*>(to[u] + (o1 - o0)) = y[u].p;
+            }
         }
     }
 }
 
 template <typename T, int V>
 static void launch_rotary(const RotaryArgs& a, bool inter, cudaStream_t st) {
-    const size_t smem = (size_t)(a.rot / 2) * sizeof(float2);
+    const int half = a.rot / 2;
+    const int warps = half <= 512 ? 4 : 1;  // each with its table in shared memory
+    const int64_t all = (int64_t)a.rows * a.parts;
+    const unsigned blocks = (unsigned)((all + warps - 1) / warps);
+    const size_t smem = (size_t)warps * half * sizeof(float2);
     if (inter)
-        rotary_kernel<T, V, true><<<(unsigned)a.rows, kRotaryThreads, smem, st>>>(a);
+        rotary_kernel<T, V, true><<<blocks, warps * 32, smem, st>>>(a);
     else
-        rotary_kernel<T, V, false><<<(unsigned)a.rows, kRotaryThreads, smem, st>>>(a);
+        rotary_kernel<T, V, false><<<blocks, warps * 32, smem, st>>>(a);
 }
 
 // 16-byte runs fit when every vector starts on one and pairs and the rest come
@@ -125,7 +200,14 @@ static void dispatch_rotary(RotaryArgs a, bool inter, cudaStream_t st) {
     const int V = wide ? kV : 1;
     a.turn_chunks = a.rot / 2 / V;
     a.chunks = a.turn_chunks + (a.dim - a.rot + 2 * V - 1) / (2 * V);
-    a.by_chunks = FastDiv((uint32_t)a.chunks);
+    a.lanes = 1;
+    while (a.lanes < 32 && a.lanes < a.chunks) a.lanes *= 2;
+    // few rows: several warps share one, as long as each has heads of its own
+    const int steps = (a.heads + 32 / a.lanes - 1) / (32 / a.lanes);
+    a.parts = 1;
+    while (a.parts * 2 <= steps && (int64_t)a.rows * a.parts < 2048) a.parts *= 2;
+    a.by_tokens = FastDiv((uint32_t)a.tokens);
+    a.by_parts = FastDiv((uint32_t)a.parts);
     if (wide)
         launch_rotary<T, kV>(a, inter, st);
     else
@@ -180,8 +262,8 @@ extern "C" chm_status chm_rotary(const chm_heads* in, const chm_heads* out, int3
     if (flags & ~(CHM_ROTARY_INTERLEAVED | CHM_ROTARY_INVERSE)) return refuse("rotary: unknown flag");
     RotaryArgs a{};
     for (int i = 0; i < n; ++i) {
-        if (in[i].heads < 0 || in[i].heads != out[i].heads || in[i].heads > (1 << 16))
-            return refuse("rotary: heads of in and out must agree, at most 65536");
+        if (in[i].heads < 0 || in[i].heads != out[i].heads || in[i].heads > (1 << 14))
+            return refuse("rotary: heads of in and out must agree, at most 16384");
         a.set[i] = HeadsView{in[i].data,         out[i].data,         in[i].batch_stride,  in[i].token_stride,
                              in[i].head_stride,  out[i].batch_stride, out[i].token_stride, out[i].head_stride};
         a.heads += in[i].heads;
@@ -201,8 +283,8 @@ extern "C" chm_status chm_rotary(const chm_heads* in, const chm_heads* out, int3
     a.freqs = freqs;
     a.scale = scale;
     a.sign = flags & CHM_ROTARY_INVERSE ? -1.0f : 1.0f;
-    a.rows = batch * tokens;
-    a.tokens = tokens;
+    a.rows = (int32_t)(batch * tokens);
+    a.tokens = (int32_t)tokens;
     const bool inter = flags & CHM_ROTARY_INTERLEAVED;
     cudaStream_t st = (cudaStream_t)stream;
     if (type == CHM_FP32)
