@@ -32,9 +32,7 @@ KINDS = {"plain": 0, "linear": 1, "base": 2, "parts": 3}
 
 
 def _run(stream, x, call, *args):
-    """call(*args), on `stream` where one is given (its device is x's)."""
-    if stream is None:
-        return call(*args)
+    """call(*args) on `stream` (its device is x's)."""
     if isinstance(x, torch.Tensor) and x.is_cuda and stream.device != x.device:
         raise ValueError(f"the stream is on {stream.device}, not on {x.device}")
     with torch.cuda.stream(stream):
@@ -73,6 +71,8 @@ def rotary(q, k, positions, freqs, *, interleaved=False, inverse=False, scale=1.
     back: the gradient with respect to q and k of the outputs' gradients, with
     the same scale.  q_out / k_out may be q and k themselves, but not overlap
     them in any other way.  Returns (q_out, k_out)."""
+    if stream is None:
+        return _g.rotary(q, k, positions, freqs, interleaved, inverse, scale, q_out, k_out)
     return _run(stream, q, _g.rotary, q, k, positions, freqs, interleaved, inverse, scale, q_out, k_out)
 
 
@@ -81,6 +81,8 @@ def cache_write(k, v, slots, k_pages, v_pages, k_scale=None, v_scale=None, *, st
     float16 or bfloat16) to slots [tokens] (int64) of the cache; int8 and
     float8_e4m3fn pages get codes and one scale per vector (chm_cache_write).
     A slot outside the cache is skipped.  No slot may stand twice."""
+    if stream is None:
+        return _g.cache_write(k, v, slots, k_pages, v_pages, k_scale, v_scale)
     return _run(stream, k, _g.cache_write, k, v, slots, k_pages, v_pages, k_scale, v_scale)
 
 
@@ -89,6 +91,8 @@ def cache_read(slots, k_pages, v_pages, k_scale=None, v_scale=None, *, dtype=tor
     """Keys and values [tokens, heads, dim] of slots [tokens] (int64), as the
     values the cache holds, rounded to `dtype`.  A slot outside the cache
     reads as zeros.  Returns (k, v)."""
+    if stream is None:
+        return _g.cache_read(slots, k_pages, v_pages, k_scale, v_scale, dtype, k_out, v_out)
     return _run(stream, k_pages, _g.cache_read, slots, k_pages, v_pages, k_scale, v_scale, dtype, k_out, v_out)
 
 
@@ -105,6 +109,9 @@ def paged_attention(q, k_pages, v_pages, tables, lens, k_scale=None, v_scale=Non
     cache NaN (chm_paged_attention).  `workspace`: a uint8 tensor of
     paged_attention_workspace bytes for callers that keep one; calls that may
     overlap, captured graphs among them, each need their own."""
+    if stream is None:
+        return _g.paged_attention(q, k_pages, v_pages, k_scale, v_scale, tables, lens, starts, scale, out, lse,
+                                  workspace)
     return _run(stream, q, _g.paged_attention, q, k_pages, v_pages, k_scale, v_scale, tables, lens, starts, scale,
                 out, lse, workspace)
 

@@ -147,7 +147,7 @@ def build_generation():
                                                           "-I" + sysconfig.get_paths()["include"]]
         _run([_cxx(), "-std=c++17", "-O2", "-fPIC", "-shared", "-o", mod, src,
               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + inc +
-             ["-L" + LIB, "-lchimera_b200", "-L" + tlib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+             ["-L" + LIB, "-lchimera_b200", "-L" + tlib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
               "-Wl,-rpath,$ORIGIN/lib"])
     return mod
 

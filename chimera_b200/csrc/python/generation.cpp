@@ -10,6 +10,8 @@
 #include <ATen/ATen.h>
 #include <ATen/Functions.h>
 #include <ATen/core/grad_mode.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -73,7 +75,8 @@ chm_heads heads_of(const Tensor& x, const char* name, bool batch, bool token) {
 
 // An output given by the caller, or a new one.
 Tensor output(PyObject* o, c10::IntArrayRef shape, ScalarType type, c10::Device device, const char* name) {
-    if (o == Py_None) return at::empty(shape, at::TensorOptions().dtype(type).device(device));
+    // (not at::empty: its dispatch is a third of a small call)
+    if (o == Py_None) return at::detail::empty_cuda(shape, type, device, std::nullopt);
     const Tensor& x = tensor_on(device, o, name);
     TORCH_CHECK_VALUE(x.sizes() == shape && x.scalar_type() == type, name, " must be ", c10::toString(type),
                       " of shape ", shape);
@@ -292,17 +295,22 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     TORCH_CHECK_VALUE(lse.is_contiguous(), "lse must be contiguous");
     const chm_heads qh = heads_of(q, "q", true, false), oh = heads_of(out, "out", true, false);
     const size_t need = chm_paged_attention_workspace_bytes(&c, batch, (int32_t)heads, width);
-    Tensor ws;
+    c10::DataPtr own;  // back to the allocator at the end: it gives the memory out again on this stream
+    void* ws;
+    size_t ws_bytes = need;
     if (a[11] == Py_None) {
-        ws = at::empty({(int64_t)need}, at::TensorOptions().dtype(ScalarType::Byte).device(dev));
+        own = c10::cuda::CUDACachingAllocator::get()->allocate(need);
+        ws = own.get();
     } else {
-        ws = tensor_on(dev, a[11], "workspace");
-        TORCH_CHECK_VALUE(ws.scalar_type() == ScalarType::Byte && ws.is_contiguous() && (size_t)ws.numel() >= need &&
-                              (uintptr_t)ws.data_ptr() % 256 == 0,
+        const Tensor& x = tensor_on(dev, a[11], "workspace");
+        ws = x.data_ptr();
+        ws_bytes = (size_t)x.numel();
+        TORCH_CHECK_VALUE(x.scalar_type() == ScalarType::Byte && x.is_contiguous() && ws_bytes >= need &&
+                              (uintptr_t)ws % 256 == 0,
                           "workspace must be contiguous uint8, 256-byte aligned, of ", need, " bytes or more");
     }
     check(chm_paged_attention(&c, &qh, &oh, type, batch, tables.data_ptr<int32_t>(), tables.stride(0), width, bounds[0],
-                              bounds[1], scale, lse.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(),
+                              bounds[1], scale, lse.data_ptr<float>(), ws, ws_bytes,
                               stream_of(dev)),
           "paged_attention");
     PyObject* r0 = a[9] != Py_None ? Py_NewRef(a[9]) : THPVariable_Wrap(out);
