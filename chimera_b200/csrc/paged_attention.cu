@@ -231,19 +231,19 @@ struct Shape {
     static constexpr int kHeads = 8 * NT;
     // blocks per SM that the registers (the output tiles) leave room for
     static constexpr int kResident = DMAX * kBytes > 256 ? 1 : DMAX > 128 || NT > 1 ? 2 : 3;
-    // A warp's copies in flight: kStages steps of keys and of values, which fill
-    // the shared memory that the resident blocks have, about 190 KB per SM.
+    // A warp's ring: kSlots copies of a step's keys or of its values, in turn, are on their
+    // way or in use.  8 KB per warp stream at 6.7 TB/s with 12 warps per SM; 12 KB cost the
+    // long sequence 66 us in place of 64.
     static constexpr int kSlot = kTok * DMAX * kBytes;
-    static constexpr int kStages = (kResident == 3 ? 8192 : kResident == 2 ? 12288 : 16384) / kSlot;
-    // shared memory: q as operand registers, factors of its rows, rings, scales; at a
-    // segment's end the warps' parts take the place of the rings
+    static constexpr int kSlots = (kResident == 3 ? 8192 : kResident == 2 ? 16384 : 32768) / kSlot;
+    static constexpr int kScaleSlots = kSlots / 2 + 1;  // steps whose scales are on their way or in use
+    // shared memory: q as operand registers, factors of its rows, rings, scales, the warps' parts
     static constexpr int kQ = NT * (DMAX / 32) * 512 + kHeads * 4;
-    static constexpr int kRing = kAttWarps * kStages * 2 * kSlot;
-    static constexpr int kScales = kWide ? 0 : kAttWarps * kStages * 2 * kTok * 4;
+    static constexpr int kRing = kAttWarps * kSlots * kSlot;
+    static constexpr int kScales = kWide ? 0 : kAttWarps * kScaleSlots * 2 * kTok * 4;
     static constexpr int kRow = DMAX + 4;
     static constexpr int kOut = kAttWarps * kHeads * (kRow + 2) * 4;
-    static_assert(kOut <= kRing, "the warps' parts fit in the rings");
-    static constexpr int kShared = kQ + kRing + kScales;
+    static constexpr int kShared = kQ + kRing + kScales + kOut;
     static_assert(kResident * (kShared + 1024) <= 227 * 1024, "the resident blocks' shared memory");
 };
 
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
     constexpr bool kWide = S::kWide;
     constexpr bool kHalf = KIND != CHM_BF16;  // fp16 products; 8-bit codes are fp16 numbers
     constexpr int kBytes = S::kBytes, kU = S::kU, kTok = S::kTok, kTile = S::kTile, kHeads = S::kHeads;
-    constexpr int kStages = S::kStages, kSlot = S::kSlot;
+    constexpr int kSlots = S::kSlots, kSlot = S::kSlot, kScaleSlots = S::kScaleSlots;
     constexpr int kKC = DMAX * kBytes / 64;         // 16-byte runs of a key per thread
     constexpr int kRuns = DMAX / 32;                // operand runs of q
     constexpr int kE = DMAX / 8;                    // value elements per thread and token
@@ -271,23 +271,24 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
     extern __shared__ __align__(16) uint8_t smem[];
     uint4(*s_q)[kRuns][32] = reinterpret_cast<uint4(*)[kRuns][32]>(smem);
     float* const s_f = reinterpret_cast<float*>(smem + NT * kRuns * 512);
-    float(*s_o)[kHeads][kRow] = reinterpret_cast<float(*)[kHeads][kRow]>(smem + S::kQ);
-    float(*s_m)[kHeads] = reinterpret_cast<float(*)[kHeads]>(smem + S::kQ + kAttWarps * kHeads * kRow * 4);
+    uint8_t* const s_parts = smem + S::kQ + S::kRing + S::kScales;
+    float(*s_o)[kHeads][kRow] = reinterpret_cast<float(*)[kHeads][kRow]>(s_parts);
+    float(*s_m)[kHeads] = reinterpret_cast<float(*)[kHeads]>(s_parts + kAttWarps * kHeads * kRow * 4);
     float(*s_l)[kHeads] = s_m + kAttWarps;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int dim = a.c.dim;
-    // This warp's ring: per stage the keys, then the values.  Keys: a lane's own 16 bytes in
-    // a row of 512, so that it reads back what it copied.  Values: eight lanes copy 128
+    // This warp's ring: the keys of a step, its values, the next step's keys and so on, a slot
+    // each.  Keys: a lane's own 16 bytes in a row of 512.  Values: eight lanes copy 128
     // bytes of a token (a row of four tokens, or of eight 64-byte ones, is one copy of 512);
     // by lane they would go to memory a sector at a time, which halves the bandwidth (3.7
     // against 6.7 TB/s).  Lane (g, t) then finds its run in line t, 16-byte places turned by
     // 2t so that neither side has bank conflicts.
-    const uint8_t* const ring = smem + S::kQ + warp * (kStages * 2 * kSlot);
-    const float* const scales = reinterpret_cast<const float*>(smem + S::kQ + S::kRing) + warp * (kStages * 2 * kTok);
+    const uint8_t* const ring = smem + S::kQ + warp * (kSlots * kSlot);
+    const float* const scales = reinterpret_cast<const float*>(smem + S::kQ + S::kRing) + warp * (kScaleSlots * 2 * kTok);
     const uint32_t ring_k = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
     const int vt = kVB == 16 ? lane >> 3 : lane >> 2;  // the token a lane copies, of kVT
     const int vc = kVB == 16 ? lane & 7 : lane & 3;    // and its 16 bytes of it
-    const uint32_t ring_v = (uint32_t)__cvta_generic_to_shared(ring) + kSlot +
+    const uint32_t ring_v = (uint32_t)__cvta_generic_to_shared(ring) +
                             (kVB == 16 ? vt * 8 + (vc ^ (2 * vt)) : (vt >> 1) * 8 + (((vt & 1) * 4 + vc) ^ (vt & 6))) * 16;
     // where lane (g, t) reads the values of its first and second token of eight
     const int run_v0 = kVB == 16 ? (t * 8 + (g ^ (2 * t))) * 16 : t * 128 + ((g >> 1) ^ (2 * t)) * 16 + (g & 1) * 8;
@@ -329,117 +330,389 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
     }
     Range r = sequence_range(a, b);
 
-    for (int piece = 0; u < u1; ++piece) {
-        const int in_seq = u - before;
-        const int seg = in_seq / r.units;
-        const int unit0 = in_seq - seg * r.units;
-        const int unit1 = min(r.units, unit0 + (u1 - u));
-        const bool whole = unit1 - unit0 == r.units;
-        if (threadIdx.x == 0) {
-            if (piece == 0) a.boundaries[blockIdx.x] = Boundary{b, seg, u - unit0, r.units};
-            if (in_seq == 0) a.before[b] = before;
+    struct Piece {
+        int b, h0, nh;  // its sequence, first query head, query heads
+        int head;       // key head
+        int first, end;
+        bool whole, bad;
+    } now{}, next{};
+    // Token `pos` of the range, one per lane: its page, then its place and scales.
+    auto page_of = [&](const Piece& it, int pos) {
+        return pos < it.end ? a.tables[it.b * a.table_stride + a.by_page.div((uint32_t)pos)] : 0;
+    };
+    uint32_t at = kNowhere;  // of this lane's token of the newest step, in 16 bytes
+    bool full = false;       // all the step's tokens are there, in their whole width
+    auto place = [&](Piece& it, int pos, int page, int slot) {
+        at = kNowhere;
+        int64_t scale = 0;
+        if (pos < it.end) {
+            if (page < 0 || page >= a.c.num_pages) {
+                it.bad = true;
+            } else {
+                const uint32_t within = (uint32_t)pos - a.by_page.div((uint32_t)pos) * (uint32_t)a.c.page_size;
+                at = (uint32_t)page * a.page16 + (uint32_t)it.head * a.head16 + within * a.token16;
+                if (!kWide) scale = ((int64_t)page * a.c.heads + it.head) * a.c.page_size + within;
+            }
         }
-        const int head = seg / a.blocks;
-        const int h0 = head * a.group + (seg - head * a.blocks) * kHeads;  // first query head
-        const int nh = min(kHeads, (head + 1) * a.group - h0);
-        const int32_t* table = a.tables + b * a.table_stride;
-        const int first = r.first + max(unit0 - a.start_units, 0) * a.unit_tokens;
-        const int end = unit1 == r.units ? r.end : r.first + max(unit1 - a.start_units, 0) * a.unit_tokens;
-        bool bad = r.bad;
-
-        // Token `pos` of the range, one per lane: its page, then its place and scales.
-        auto page_of = [&](int pos) { return pos < end ? table[a.by_page.div((uint32_t)pos)] : 0; };
-        uint32_t at = kNowhere;  // of this lane's token of the newest step, in 16 bytes
-        bool full = false;       // all the step's tokens are there, in their whole width
-        auto place = [&](int pos, int page, int stage) {
-            at = kNowhere;
-            int64_t scale = 0;
-            if (pos < end) {
-                if (page < 0 || page >= a.c.num_pages) {
-                    bad = true;
-                } else {
-                    const uint32_t within = (uint32_t)pos - a.by_page.div((uint32_t)pos) * (uint32_t)a.c.page_size;
-                    at = (uint32_t)page * a.page16 + (uint32_t)head * a.head16 + within * a.token16;
-                    if (!kWide) scale = ((int64_t)page * a.c.heads + head) * a.c.page_size + within;
+        if (!kWide && lane < kTok) {
+            copy_async_if<4>(scales_at + slot * (2 * kTok * 4), a.c.k_scale + scale, at != kNowhere);
+            copy_async_if<4>(scales_at + slot * (2 * kTok * 4) + kTok * 4, a.c.v_scale + scale, at != kNowhere);
+        }
+        full = __all_sync(0xffffffffu, at != kNowhere) && dim == DMAX;
+    };
+    auto copy_keys = [&](int slot) {
+        const uint32_t to = ring_k + slot * kSlot;
+#pragma unroll
+        for (int i = 0; i < 2 * kU; ++i) {
+            const uint32_t x = __shfl_sync(0xffffffffu, at, i * 8 + g);
+            const char* p = kbase + (uint64_t)x * 16;
+            if (full) {
+                copy_async<16, 0>(to + i * kKC * 512, p);
+                if (kKC > 1) copy_async<16, 64>(to + (i * kKC + 1) * 512, p);
+                if (kKC > 2) copy_async<16, 128>(to + (i * kKC + 2) * 512, p);
+                if (kKC > 3) copy_async<16, 192>(to + (i * kKC + 3) * 512, p);
+                if (kKC > 4) {
+                    copy_async<16, 256>(to + (i * kKC + 4) * 512, p);
+                    copy_async<16, 320>(to + (i * kKC + 5) * 512, p);
+                    copy_async<16, 384>(to + (i * kKC + 6) * 512, p);
+                    copy_async<16, 448>(to + (i * kKC + 7) * 512, p);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < kKC; ++c) {
+                    const bool on = x != kNowhere && c * 64 + t * 16 < dim * kBytes;
+                    copy_async_if<16>(to + (i * kKC + c) * 512, on ? p + c * 64 : kbase, on);
                 }
             }
-            if (!kWide && lane < kTok) {
-                copy_async_if<4>(scales_at + stage * (2 * kTok * 4), a.c.k_scale + scale, at != kNowhere);
-                copy_async_if<4>(scales_at + stage * (2 * kTok * 4) + kTok * 4, a.c.v_scale + scale, at != kNowhere);
-            }
-            full = __all_sync(0xffffffffu, at != kNowhere) && dim == DMAX;
-        };
-        auto copy_keys = [&](int stage) {
-            const uint32_t to = ring_k + stage * 2 * kSlot;
+        }
+    };
+    auto copy_values = [&](int slot) {
+        const uint32_t to = ring_v + slot * kSlot;
 #pragma unroll
-            for (int i = 0; i < 2 * kU; ++i) {
-                const uint32_t x = __shfl_sync(0xffffffffu, at, i * 8 + g);
-                const char* p = kbase + (uint64_t)x * 16;
-                if (full) {
-                    copy_async<16, 0>(to + i * kKC * 512, p);
-                    if (kKC > 1) copy_async<16, 64>(to + (i * kKC + 1) * 512, p);
-                    if (kKC > 2) copy_async<16, 128>(to + (i * kKC + 2) * 512, p);
-                    if (kKC > 3) copy_async<16, 192>(to + (i * kKC + 3) * 512, p);
-                    if (kKC > 4) {
-                        copy_async<16, 256>(to + (i * kKC + 4) * 512, p);
-                        copy_async<16, 320>(to + (i * kKC + 5) * 512, p);
-                        copy_async<16, 384>(to + (i * kKC + 6) * 512, p);
-                        copy_async<16, 448>(to + (i * kKC + 7) * 512, p);
-                    }
-                } else {
+        for (int i = 0; i < kTok / kVT; ++i) {
+            // 128-byte runs: tokens 2t or 2t + 1 of eight, as lanes t need them together
+            const int src = kVB == 16 ? (i >> 1) * 8 + 2 * vt + (i & 1) : i * 8 + vt;
+            const uint32_t x = __shfl_sync(0xffffffffu, at, src);
+            const char* p = vbase + (uint64_t)x * 16;
+            if (full) {
+                copy_async<16, 0>(to + i * kVC * 512, p);
+                if (kVC > 1) copy_async<16, 128>(to + (i * kVC + 1) * 512, p);
+                if (kVC > 2) {
+                    copy_async<16, 256>(to + (i * kVC + 2) * 512, p);
+                    copy_async<16, 384>(to + (i * kVC + 3) * 512, p);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < kVC; ++c) {
+                    const bool on = x != kNowhere && c * 128 + vc * 16 < dim * kBytes;
+                    copy_async_if<16>(to + (i * kVC + c) * 512, on ? p + c * 128 : vbase, on);
+                }
+            }
+        }
+    };
+
+    int pos = 0;           // this lane's token of the newest step
+    int next_page = 0;     // and its page, of the step after
+    int newest = 0;        // the newest step's first token
+    bool live = false;     // whether that step has tokens
+    int scale_in = 0;      // where the newest step's scales go
+    // The next step of `it`: where its tokens are, its scales and keys on their way.
+    auto next_keys = [&](Piece& it, int slot) {
+        pos += kTile, newest += kTile;
+        live = newest < it.end;
+        scale_in = scale_in + 1 == kScaleSlots ? 0 : scale_in + 1;
+        if (live) {
+            const int page = next_page;
+            next_page = page_of(it, pos + kTile);
+            place(it, pos, page, scale_in);
+            copy_keys(slot);
+        }
+        copies_commit();
+    };
+    auto its_values = [&](int slot) {
+        if (live) copy_values(slot);
+        copies_commit();
+    };
+
+    // ---- segment by segment; the next one's first copies are on their way while this one's
+    // parts are joined
+    for (int piece = -1;; ++piece) {
+        float o[NT][kM][4] = {};
+        float m[NT][2], l[NT][2];  // references and sums of this lane's columns
+#pragma unroll
+        for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.0f;
+        if (piece >= 0) {
+            float qf[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) qf[n][e] = kWide ? a.scale_log2 : s_f[n * 8 + 2 * t + e];
+
+            // The copies run kSlots half steps ahead: what has just been read makes room for the
+            // newest step's values or the next one's keys.
+            int slot = 0, scale_out = 0;
+            for (int base = now.first + warp * kTok; base < now.end; base += kTile) {
+                const uint8_t* const keys = ring + slot * kSlot + lane * 16;
+                copies_wait<kSlots - 1>();
+                __syncwarp();
+                // ---- scores
+                float sc[NT][kU][4] = {};
+#pragma unroll
+                for (int i = 0; i < kU; ++i)
 #pragma unroll
                     for (int c = 0; c < kKC; ++c) {
-                        const bool on = x != kNowhere && c * 64 + t * 16 < dim * kBytes;
-                        copy_async_if<16>(to + (i * kKC + c) * 512, on ? p + c * 64 : kbase, on);
+                        const uint4 r0 = *reinterpret_cast<const uint4*>(keys + (i * 2 * kKC + c) * 512);
+                        const uint4 r1 = *reinterpret_cast<const uint4*>(keys + ((i * 2 + 1) * kKC + c) * 512);
+                        const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
+                        // pairs of the run: 4 words of a 16-bit cache, 8 pairs of codes
+#pragma unroll
+                        for (int j = 0; j < (kWide ? 1 : 2); ++j) {
+                            uint32_t p0[4], p1[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                if (kWide)
+                                    p0[e] = w0[e], p1[e] = w1[e];
+                                else if (e % 2 == 0) {
+                                    codes_of_word<KIND>(w0[j * 2 + e / 2], p0[e], p0[e + 1]);
+                                    codes_of_word<KIND>(w1[j * 2 + e / 2], p1[e], p1[e + 1]);
+                                }
+                            }
+                            const int run = kWide ? c : c * 2 + j;
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                const uint4 bq = s_q[n][run][lane];
+                                mma<kHalf>(sc[n][i], p0[0], p1[0], p0[1], p1[1], bq.x, bq.y);
+                                mma<kHalf>(sc[n][i], p0[2], p1[2], p0[3], p1[3], bq.z, bq.w);
+                            }
+                        }
+                    }
+                // ---- scaled; tokens past the end get weight zero
+                float vs[kU][2], lv[kU][2];
+                if (!kWide) {
+#pragma unroll
+                    for (int i = 0; i < kU; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int src = i * 16 + h * 8 + g;
+                            const float ks = scales[scale_out * 2 * kTok + src];
+                            vs[i][h] = scales[scale_out * 2 * kTok + kTok + src];
+                            lv[i][h] = fmaxf(log2_fast(fabsf(vs[i][h])), -105.0f);  // the smallest scale written
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) sc[n][i][h * 2 + e] *= ks;
+                        }
+                    scale_out = scale_out + 1 == kScaleSlots ? 0 : scale_out + 1;
+                }
+                bool above = false;
+#pragma unroll
+                for (int i = 0; i < kU; ++i)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sc[n][i][e] *= qf[n][e & 1];
+                if (base + kTok > now.end) {
+#pragma unroll
+                    for (int i = 0; i < kU; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            if (base + i * 16 + h * 8 + g >= now.end) {
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) sc[n][i][h * 2] = sc[n][i][h * 2 + 1] = -INFINITY;
+                            }
+                }
+#pragma unroll
+                for (int i = 0; i < kU; ++i)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            above = above || (kWide ? sc[n][i][e] : sc[n][i][e] + lv[i][e >> 1]) > m[n][e & 1] + kRoom;
+                __syncwarp();  // all lanes have read the keys and scales
+                if (kSlots % 2)
+                    its_values(slot);
+                else
+                    next_keys(now, slot);
+                slot = slot + 1 == kSlots ? 0 : slot + 1;
+                // ---- the reference follows the largest exponent
+                if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float top = m[n][e] + kLead;
+#pragma unroll
+                            for (int i = 0; i < kU; ++i)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h)
+                                    top = fmaxf(top, kWide ? sc[n][i][h * 2 + e] : sc[n][i][h * 2 + e] + lv[i][h]);
+#pragma unroll
+                            for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                            top -= kLead;
+                            const float f = top > m[n][e] ? exp2_fast(m[n][e] - top) : 1.0f;
+                            m[n][e] = fmaxf(top, m[n][e]);
+                            l[n][e] *= f;
+#pragma unroll
+                            for (int i = 0; i < kM; ++i) o[n][i][e] *= f, o[n][i][2 + e] *= f;
+                        }
+                }
+                // ---- weights as the operand of the second product, in two 16-bit terms
+                uint32_t ph[NT][kU][2], pl[NT][kU][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float m0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
+#pragma unroll
+                    for (int i = 0; i < kU; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            float p0 = exp2_fast(sc[n][i][h * 2] - m0), p1 = exp2_fast(sc[n][i][h * 2 + 1] - m1);
+                            l[n][0] += p0, l[n][1] += p1;
+                            if (!kWide) p0 *= vs[i][h], p1 *= vs[i][h];
+                            const uint32_t hi = pack16<kHalf>(p0, p1);
+                            const float2 y = unpack16<kHalf>(hi);
+                            ph[n][i][h] = transpose8(hi);
+                            pl[n][i][h] = transpose8(pack16<kHalf>(p0 - y.x, p1 - y.y));
+                        }
+                }
+                // ---- values
+                const uint8_t* const values = ring + slot * kSlot;
+                copies_wait<kSlots - 1>();
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < kU; ++i) {
+                    uint32_t vr[4][kVC * kVB / 4];
+#pragma unroll
+                    for (int h = 0; h < 4; ++h)
+#pragma unroll
+                        for (int c = 0; c < kVC; ++c) {
+                            if (kVB == 16) {
+                                const uint4 w = *reinterpret_cast<const uint4*>(values + ((i * 4 + h) * kVC + c) * 512 + run_v0);
+                                vr[h][c * 4] = w.x, vr[h][c * 4 + 1] = w.y, vr[h][c * 4 + 2] = w.z, vr[h][c * 4 + 3] = w.w;
+                            } else {
+                                const uint2 w = *reinterpret_cast<const uint2*>(values + (i * 2 + (h >> 1)) * 512 +
+                                                                                (h & 1 ? run_v1 : run_v0));
+                                vr[h][0] = w.x, vr[h][1] = w.y;
+                            }
+                        }
+#pragma unroll
+                    for (int j = 0; j < kM; ++j) {
+                        uint32_t f[4];
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {  // row block h & 1, tokens h >> 1
+                            const int x = j + (h & 1) * kM;
+                            const uint32_t* v0 = vr[(h >> 1) * 2];
+                            const uint32_t* v1 = vr[(h >> 1) * 2 + 1];
+                            if (kWide)
+                                f[h] = __byte_perm(v0[x / 2], v1[x / 2], (x & 1) ? 0x7632 : 0x5410);
+                            else
+                                f[h] = codes_of_pair<KIND>(v0[x / 4], v1[x / 4], x & 3);
+                        }
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            mma<kHalf>(o[n][j], f[0], f[1], f[2], f[3], ph[n][i][0], ph[n][i][1]);
+                            mma<kHalf>(o[n][j], f[0], f[1], f[2], f[3], pl[n][i][0], pl[n][i][1]);
+                        }
                     }
                 }
+                __syncwarp();
+                if (kSlots % 2)
+                    next_keys(now, slot);
+                else
+                    its_values(slot);
+                slot = slot + 1 == kSlots ? 0 : slot + 1;
             }
-        };
-        auto copy_values = [&](int stage) {
-            const uint32_t to = ring_v + stage * 2 * kSlot;
-#pragma unroll
-            for (int i = 0; i < kTok / kVT; ++i) {
-                // 128-byte runs: tokens 2t or 2t + 1 of eight, as lanes t need them together
-                const int src = kVB == 16 ? (i >> 1) * 8 + 2 * vt + (i & 1) : i * 8 + vt;
-                const uint32_t x = __shfl_sync(0xffffffffu, at, src);
-                const char* p = vbase + (uint64_t)x * 16;
-                if (full) {
-                    copy_async<16, 0>(to + i * kVC * 512, p);
-                    if (kVC > 1) copy_async<16, 128>(to + (i * kVC + 1) * 512, p);
-                    if (kVC > 2) {
-                        copy_async<16, 256>(to + (i * kVC + 2) * 512, p);
-                        copy_async<16, 384>(to + (i * kVC + 3) * 512, p);
-                    }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < kVC; ++c) {
-                        const bool on = x != kNowhere && c * 128 + vc * 16 < dim * kBytes;
-                        copy_async_if<16>(to + (i * kVC + c) * 512, on ? p + c * 128 : vbase, on);
-                    }
-                }
-            }
-        };
-
-        int pos = first + warp * kTok + lane % kTok;  // this lane's token of the newest step
-        int base = first + warp * kTok;               // the oldest step's first
-        int next_page = page_of(pos);
-#pragma unroll
-        for (int i = 0; i < kStages; ++i) {
-            const int page = next_page;
-            next_page = page_of(pos + kTile);
-            if (base + i * kTile < end) {
-                place(pos, page, i);
-                copy_keys(i);
-                copies_commit();
-                copy_values(i);
-                copies_commit();
-            } else {
-                copies_commit();
-                copies_commit();
-            }
-            pos += kTile;
+            copies_wait<0>();
         }
-
+        // ---- the next segment
+        const bool last = u >= u1;
+        if (!last) {
+            if (u == before + r.units * segs) {
+                before = u;
+                r = sequence_range(a, ++b);
+            }
+            const int in_seq = u - before;
+            const int seg = in_seq / r.units;
+            const int unit0 = in_seq - seg * r.units;
+            const int unit1 = min(r.units, unit0 + (u1 - u));
+            if (threadIdx.x == 0) {
+                if (piece < 0) a.boundaries[blockIdx.x] = Boundary{b, seg, u - unit0, r.units};
+                if (in_seq == 0) a.before[b] = before;
+            }
+            next.b = b;
+            next.head = seg / a.blocks;
+            next.h0 = next.head * a.group + (seg - next.head * a.blocks) * kHeads;
+            next.nh = min(kHeads, (next.head + 1) * a.group - next.h0);
+            next.first = r.first + max(unit0 - a.start_units, 0) * a.unit_tokens;
+            next.end = unit1 == r.units ? r.end : r.first + max(unit1 - a.start_units, 0) * a.unit_tokens;
+            next.whole = unit1 - unit0 == r.units;
+            next.bad = r.bad;
+            u += unit1 - unit0;
+        }
+        // ---- this segment's warps' parts to shared memory
+        if (piece >= 0) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float sum = l[n][e];
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+                    const int hh = n * 8 + 2 * t + e;
+                    if (g == 0) s_m[warp][hh] = m[n][e], s_l[warp][hh] = sum;
+#pragma unroll
+                    for (int x = 0; x < kE; x += 4) {
+                        const int d = kWide ? (x / 8) * 64 + g * 8 + x % 8
+                                            : kE >= 16 ? (x / 16) * 128 + g * 16 + x % 16 : g * 8 + x;
+                        const int j = x % kM, k = x / kM * 2 + e;
+                        *reinterpret_cast<float4*>(&s_o[warp][hh][d]) =
+                            make_float4(o[n][j][k], o[n][j + 1][k], o[n][j + 2][k], o[n][j + 3][k]);
+                    }
+                }
+        }
+        if (!last) {
+            newest = next.first + warp * kTok - kTile;
+            pos = newest + lane % kTok;
+            next_page = page_of(next, pos + kTile);
+            scale_in = -1;
+#pragma unroll
+            for (int n = 0; n < kSlots; ++n) {
+                if (n % 2 == 0)
+                    next_keys(next, n);
+                else
+                    its_values(n);
+            }
+        }
+        if (piece >= 0) {
+            const bool bad = __syncthreads_or(now.bad);
+            for (int hh = warp; hh < now.nh; hh += kAttWarps) {
+                float top = -INFINITY, sum = 0.0f, f[kAttWarps];
+#pragma unroll
+                for (int w = 0; w < kAttWarps; ++w) top = fmaxf(top, s_m[w][hh]);
+#pragma unroll
+                for (int w = 0; w < kAttWarps; ++w) {
+                    f[w] = s_m[w][hh] == -INFINITY ? 0.0f : exp2_fast(s_m[w][hh] - top);
+                    sum += f[w] * s_l[w][hh];
+                }
+                if (bad) sum = __int_as_float(0x7FC00000);
+                float* part = part_row<DMAX>(a.parts, 2 * blockIdx.x + (piece > 0), kHeads, hh);
+                for (int d = lane; d < dim; d += 32) {
+                    float acc = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < kAttWarps; ++w) acc += f[w] * s_o[w][hh][d];
+                    if (now.whole)
+                        store_row(a, now.b, now.h0 + hh, d, sum == 0.0f ? 0.0f : bad ? sum : acc / sum);
+                    else
+                        part[d] = acc;
+                }
+                if (lane == 0) {
+                    if (!now.whole)
+                        part[DMAX] = top, part[DMAX + 1] = sum;
+                    else if (a.lse)
+                        a.lse[(int64_t)now.b * a.q_heads + now.h0 + hh] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
+                }
+            }
+        }
+        if (last) break;
         // q: lane (g, t) of a run holds the 8 elements that its key runs meet.  For an 8-bit
         // cache a row is brought by a power of two to a largest element below 2^14, so that
         // fp16 holds it (exactly but for elements below 2^-28 of the largest).
@@ -450,8 +723,8 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
             for (int h = 0; h < kHeads; h += kAttWarps * (32 / kLanes)) {
                 const int hh = h + warp * (32 / kLanes) + lane / kLanes;
                 float x[8] = {};
-                const int64_t qa = b * a.q_b + (h0 + hh) * a.q_h + d0;
-                if (hh < nh && d0 < dim) {
+                const int64_t qa = next.b * a.q_b + (next.h0 + hh) * a.q_h + d0;
+                if (hh < next.nh && d0 < dim) {
                     uint32_t w[4];
                     if (a.q_wide) {
                         const uint4 y = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + qa);
@@ -491,249 +764,7 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
             }
         }
         __syncthreads();
-        float qf[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) qf[n][e] = kWide ? a.scale_log2 : s_f[n * 8 + 2 * t + e];
-
-        float o[NT][kM][4] = {};
-        float m[NT][2], l[NT][2];  // references and sums of this lane's columns
-#pragma unroll
-        for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.0f;
-
-        // The copies run kStages steps ahead: a step's keys and values are copied into the
-        // slots that the step kStages before it has just been read from.
-        int stage = 0;
-        for (; base < end; base += kTile) {
-            const uint8_t* const keys = ring + stage * 2 * kSlot + lane * 16;
-            const uint8_t* const values = ring + stage * 2 * kSlot + kSlot;
-            const bool more = base + kStages * kTile < end;
-            const int page = next_page;
-            next_page = page_of(pos + kTile);
-            copies_wait<2 * kStages - 1>();
-            __syncwarp();
-            // ---- scores
-            float sc[NT][kU][4] = {};
-#pragma unroll
-            for (int i = 0; i < kU; ++i)
-#pragma unroll
-                for (int c = 0; c < kKC; ++c) {
-                    const uint4 r0 = *reinterpret_cast<const uint4*>(keys + (i * 2 * kKC + c) * 512);
-                    const uint4 r1 = *reinterpret_cast<const uint4*>(keys + ((i * 2 + 1) * kKC + c) * 512);
-                    const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
-                    // pairs of the run: 4 words of a 16-bit cache, 8 pairs of codes
-#pragma unroll
-                    for (int j = 0; j < (kWide ? 1 : 2); ++j) {
-                        uint32_t p0[4], p1[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            if (kWide)
-                                p0[e] = w0[e], p1[e] = w1[e];
-                            else if (e % 2 == 0) {
-                                codes_of_word<KIND>(w0[j * 2 + e / 2], p0[e], p0[e + 1]);
-                                codes_of_word<KIND>(w1[j * 2 + e / 2], p1[e], p1[e + 1]);
-                            }
-                        }
-                        const int run = kWide ? c : c * 2 + j;
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            const uint4 bq = s_q[n][run][lane];
-                            mma<kHalf>(sc[n][i], p0[0], p1[0], p0[1], p1[1], bq.x, bq.y);
-                            mma<kHalf>(sc[n][i], p0[2], p1[2], p0[3], p1[3], bq.z, bq.w);
-                        }
-                    }
-                }
-            // ---- scaled; tokens past the end get weight zero
-            float vs[kU][2], lv[kU][2];
-            if (!kWide) {
-#pragma unroll
-                for (int i = 0; i < kU; ++i)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int src = i * 16 + h * 8 + g;
-                        const float ks = scales[stage * 2 * kTok + src];
-                        vs[i][h] = scales[stage * 2 * kTok + kTok + src];
-                        lv[i][h] = fmaxf(log2_fast(fabsf(vs[i][h])), -105.0f);  // the smallest scale written
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) sc[n][i][h * 2 + e] *= ks;
-                    }
-                __syncwarp();  // the scales are read; the next step's take their place
-            }
-            bool above = false;
-#pragma unroll
-            for (int i = 0; i < kU; ++i)
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) sc[n][i][e] *= qf[n][e & 1];
-            if (base + kTok > end) {
-#pragma unroll
-                for (int i = 0; i < kU; ++i)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        if (base + i * 16 + h * 8 + g >= end) {
-#pragma unroll
-                            for (int n = 0; n < NT; ++n) sc[n][i][h * 2] = sc[n][i][h * 2 + 1] = -INFINITY;
-                        }
-            }
-#pragma unroll
-            for (int i = 0; i < kU; ++i)
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        above = above || (kWide ? sc[n][i][e] : sc[n][i][e] + lv[i][e >> 1]) > m[n][e & 1] + kRoom;
-            if (more) {
-                place(pos, page, stage);
-                copy_keys(stage);
-            }
-            copies_commit();
-            pos += kTile;
-            // ---- the reference follows the largest exponent
-            if (__any_sync(0xffffffffu, above)) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float top = m[n][e] + kLead;
-#pragma unroll
-                        for (int i = 0; i < kU; ++i)
-#pragma unroll
-                            for (int h = 0; h < 2; ++h)
-                                top = fmaxf(top, kWide ? sc[n][i][h * 2 + e] : sc[n][i][h * 2 + e] + lv[i][h]);
-#pragma unroll
-                        for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-                        top -= kLead;
-                        const float f = top > m[n][e] ? exp2_fast(m[n][e] - top) : 1.0f;
-                        m[n][e] = fmaxf(top, m[n][e]);
-                        l[n][e] *= f;
-#pragma unroll
-                        for (int i = 0; i < kM; ++i) o[n][i][e] *= f, o[n][i][2 + e] *= f;
-                    }
-            }
-            // ---- weights as the operand of the second product, in two 16-bit terms
-            uint32_t ph[NT][kU][2], pl[NT][kU][2];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const float m0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
-#pragma unroll
-                for (int i = 0; i < kU; ++i)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float p0 = exp2_fast(sc[n][i][h * 2] - m0), p1 = exp2_fast(sc[n][i][h * 2 + 1] - m1);
-                        l[n][0] += p0, l[n][1] += p1;
-                        if (!kWide) p0 *= vs[i][h], p1 *= vs[i][h];
-                        const uint32_t hi = pack16<kHalf>(p0, p1);
-                        const float2 y = unpack16<kHalf>(hi);
-                        ph[n][i][h] = transpose8(hi);
-                        pl[n][i][h] = transpose8(pack16<kHalf>(p0 - y.x, p1 - y.y));
-                    }
-            }
-            // ---- values
-            copies_wait<2 * kStages - 1>();
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < kU; ++i) {
-                uint32_t vr[4][kVC * kVB / 4];
-#pragma unroll
-                for (int h = 0; h < 4; ++h)
-#pragma unroll
-                    for (int c = 0; c < kVC; ++c) {
-                        if (kVB == 16) {
-                            const uint4 w = *reinterpret_cast<const uint4*>(values + ((i * 4 + h) * kVC + c) * 512 + run_v0);
-                            vr[h][c * 4] = w.x, vr[h][c * 4 + 1] = w.y, vr[h][c * 4 + 2] = w.z, vr[h][c * 4 + 3] = w.w;
-                        } else {
-                            const uint2 w = *reinterpret_cast<const uint2*>(values + (i * 2 + (h >> 1)) * 512 +
-                                                                            (h & 1 ? run_v1 : run_v0));
-                            vr[h][0] = w.x, vr[h][1] = w.y;
-                        }
-                    }
-#pragma unroll
-                for (int j = 0; j < kM; ++j) {
-                    uint32_t f[4];
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) {  // row block h & 1, tokens h >> 1
-                        const int x = j + (h & 1) * kM;
-                        const uint32_t* v0 = vr[(h >> 1) * 2];
-                        const uint32_t* v1 = vr[(h >> 1) * 2 + 1];
-                        if (kWide)
-                            f[h] = __byte_perm(v0[x / 2], v1[x / 2], (x & 1) ? 0x7632 : 0x5410);
-                        else
-                            f[h] = codes_of_pair<KIND>(v0[x / 4], v1[x / 4], x & 3);
-                    }
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        mma<kHalf>(o[n][j], f[0], f[1], f[2], f[3], ph[n][i][0], ph[n][i][1]);
-                        mma<kHalf>(o[n][j], f[0], f[1], f[2], f[3], pl[n][i][0], pl[n][i][1]);
-                    }
-                }
-            }
-            if (more) {
-                __syncwarp();  // all lanes have read these slots
-                copy_values(stage);
-            }
-            copies_commit();
-            stage = stage + 1 == kStages ? 0 : stage + 1;
-        }
-        copies_wait<0>();
-
-        // ---- the warps' parts joined
-        bad = __syncthreads_or(bad);
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                float sum = l[n][e];
-#pragma unroll
-                for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-                const int hh = n * 8 + 2 * t + e;
-                if (g == 0) s_m[warp][hh] = m[n][e], s_l[warp][hh] = sum;
-#pragma unroll
-                for (int x = 0; x < kE; x += 4) {
-                    const int d = kWide ? (x / 8) * 64 + g * 8 + x % 8
-                                        : kE >= 16 ? (x / 16) * 128 + g * 16 + x % 16 : g * 8 + x;
-                    const int j = x % kM, k = x / kM * 2 + e;
-                    *reinterpret_cast<float4*>(&s_o[warp][hh][d]) =
-                        make_float4(o[n][j][k], o[n][j + 1][k], o[n][j + 2][k], o[n][j + 3][k]);
-                }
-            }
-        __syncthreads();
-        for (int hh = warp; hh < nh; hh += kAttWarps) {
-            float top = -INFINITY, sum = 0.0f, f[kAttWarps];
-#pragma unroll
-            for (int w = 0; w < kAttWarps; ++w) top = fmaxf(top, s_m[w][hh]);
-#pragma unroll
-            for (int w = 0; w < kAttWarps; ++w) {
-                f[w] = s_m[w][hh] == -INFINITY ? 0.0f : exp2_fast(s_m[w][hh] - top);
-                sum += f[w] * s_l[w][hh];
-            }
-            if (bad) sum = __int_as_float(0x7FC00000);
-            float* part = part_row<DMAX>(a.parts, 2 * blockIdx.x + (piece > 0), kHeads, hh);
-            for (int d = lane; d < dim; d += 32) {
-                float acc = 0.0f;
-#pragma unroll
-                for (int w = 0; w < kAttWarps; ++w) acc += f[w] * s_o[w][hh][d];
-                if (whole)
-                    store_row(a, b, h0 + hh, d, sum == 0.0f ? 0.0f : bad ? sum : acc / sum);
-                else
-                    part[d] = acc;
-            }
-            if (lane == 0) {
-                if (!whole)
-                    part[DMAX] = top, part[DMAX + 1] = sum;
-                else if (a.lse)
-                    a.lse[(int64_t)b * a.q_heads + h0 + hh] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
-            }
-        }
-        __syncthreads();  // the parts are read; the next segment's copies take their place
-        u += unit1 - unit0;
-        if (u == before + r.units * segs && u < u1) {
-            before = u;
-            r = sequence_range(a, ++b);
-        }
+        now = next;
     }
 }
 
@@ -748,7 +779,7 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const AttA
     constexpr int kV = DMAX / 32;   // elements per lane
     constexpr int kAhead = kV > 4 ? 4 : 8;  // parts on their way per warp
     __shared__ float s_acc[kJoinThreads / 32][DMAX];
-    __shared__ float s_sum[kJoinThreads / 32];
+    __shared__ float s_sum[kJoinThreads / 32], s_top[kJoinThreads / 32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const Plan plan = *a.plan;
@@ -773,43 +804,59 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const AttA
     if (h0 + hh >= (head + 1) * a.group) return;
     const int odd = c0 * plan.per != s.first;  // whether the first part is its block's second slot
     auto part = [&](int i) { return part_row<DMAX>(a.parts, 2 * i + (i == c0 ? odd : 0), kHeads, hh); };
-    // each warp takes every warps-th part; the largest reference first, then the sums
-    float top = -INFINITY;
-    for (int i = c0 + lane; i <= c1; i += 32) top = fmaxf(top, part(i)[DMAX]);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    float sum = 0.0f, acc[kV] = {};
+    // each warp takes every warps-th part, kAhead of them on their way at once
+    float top = -INFINITY, sum = 0.0f, acc[kV] = {};
     for (int i = c0 + warp; i <= c1; i += warps * kAhead) {
-        float x[kAhead][kV], w[kAhead], l[kAhead];
+        float x[kAhead][kV], m[kAhead], l[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const bool on = i + j * warps <= c1;
             const float* p = part(on ? i + j * warps : i);
-            const float m = p[DMAX];
-            w[j] = on && m != -INFINITY ? exp2_fast(m - top) : 0.0f;
+            m[j] = on ? p[DMAX] : -INFINITY;
             l[j] = on ? p[DMAX + 1] : 0.0f;
 #pragma unroll
             for (int v = 0; v < kV; ++v) x[j][v] = on ? p[v * 32 + lane] : 0.0f;
         }
+        float now = top;
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) now = fmaxf(now, m[j]);
+        const float f = top == now ? 1.0f : exp2_fast(top - now);
+        top = now;
+        sum *= f;
+#pragma unroll
+        for (int v = 0; v < kV; ++v) acc[v] *= f;
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
-            sum += l[j] * w[j];
+            const float w = m[j] == -INFINITY ? 0.0f : exp2_fast(m[j] - top);
+            sum += l[j] * w;
 #pragma unroll
-            for (int v = 0; v < kV; ++v) acc[v] += x[j][v] * w[j];
+            for (int v = 0; v < kV; ++v) acc[v] += x[j][v] * w;
         }
     }
+    if (warps > 1) {
 #pragma unroll
-    for (int v = 0; v < kV; ++v) s_acc[warp][v * 32 + lane] = acc[v];
-    if (lane == 0) s_sum[warp] = sum;
-    __syncthreads();
-    sum = 0.0f;
-    for (int w = 0; w < warps; ++w) sum += s_sum[w];
-    for (int d = threadIdx.x; d < a.c.dim; d += blockDim.x) {
-        float y = 0.0f;
-        for (int w = 0; w < warps; ++w) y += s_acc[w][d];
-        store_row(a, s.seq, h0 + hh, d, sum == 0.0f ? 0.0f : sum != sum ? sum : y / sum);
+        for (int v = 0; v < kV; ++v) s_acc[warp][v * 32 + lane] = acc[v];
+        if (lane == 0) s_sum[warp] = sum, s_top[warp] = top;
+        __syncthreads();
+        if (warp > 0) return;
+        float all = top;
+        for (int w = 1; w < warps; ++w) all = fmaxf(all, s_top[w]);
+        sum = 0.0f;
+#pragma unroll
+        for (int v = 0; v < kV; ++v) acc[v] = 0.0f;
+        for (int w = 0; w < warps; ++w) {
+            const float f = s_top[w] == -INFINITY ? 0.0f : exp2_fast(s_top[w] - all);
+            sum += f * s_sum[w];
+#pragma unroll
+            for (int v = 0; v < kV; ++v) acc[v] += f * s_acc[w][v * 32 + lane];
+        }
+        top = all;
     }
-    if (threadIdx.x == 0 && a.lse)
+#pragma unroll
+    for (int v = 0; v < kV; ++v)
+        if (v * 32 + lane < a.c.dim)
+            store_row(a, s.seq, h0 + hh, v * 32 + lane, sum == 0.0f ? 0.0f : sum != sum ? sum : acc[v] / sum);
+    if (lane == 0 && a.lse)
         a.lse[(int64_t)s.seq * a.q_heads + h0 + hh] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
@@ -905,11 +952,14 @@ struct Launch {
         paged_attention_kernel<DMAX, KIND, NT><<<(unsigned)y.blocks, kAttThreads, S::kShared, st>>>(a);
         CHM_TRY(launch_status("paged_attention_kernel"));
         if (!y.joins || y.blocks < 2) return CHM_OK;
-        // The join's blocks start while the main kernel's last ones run, and wait for its
-        // end.  Few segments have many parts each: more warps to add them.
+        // The join's blocks start while the main kernel's last ones run, and wait for its end.
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3((unsigned)(a.join_segments ? segments : y.blocks - 1), (unsigned)std::min(S::kHeads, a.group));
-        cfg.blockDim = dim3(segments * 32 < y.blocks ? kJoinThreads : 64);
+        // a warp has 8 parts on their way: warps enough for eight rounds of the most a segment
+        // can have (64 sequences up to 4,096 tokens, 128 long documents: one warp 99.6 and 37.4
+        // us, four 100.0 and 38.1; one sequence of 262,144: eight)
+        const int64_t most = std::min<int64_t>(y.blocks, y.units / segments);
+        cfg.blockDim = dim3((unsigned)std::min<int64_t>(kJoinThreads, 32 * ((most + 63) / 64)));
         cfg.stream = st;
         cudaLaunchAttribute attr{};
         attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
