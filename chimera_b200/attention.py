@@ -102,7 +102,8 @@ def paged_attention(q, k_pages, v_pages, tables, lens, k_scale=None, v_scale=Non
     (float16 or bfloat16, a 16-bit cache's own type), over tokens
     starts[b] <= j < lens[b] of its sequence (int32 [batch]; starts default to
     0), token j in page tables[b, j // page_size] (int32 [batch, width]).
-    Query heads share key heads evenly.  scale defaults to dim ** -0.5.
+    Query heads share key heads evenly.  scale defaults to dim ** -0.5.  out may
+    be q itself.
 
     Returns (out like q, lse float32 [batch, q_heads]); a row with nothing to
     attend to gets zeros and -inf, one whose table or length does not fit the

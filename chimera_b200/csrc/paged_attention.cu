@@ -935,6 +935,10 @@ struct Launch {
         Arena arena(ws, ws_bytes);
         carve(arena, y, &a, a.batch);
         if (arena.overflow) return CHM_ERR_CAPACITY;
+        if (a.c.num_pages == 0) {  // copies of nothing still name an address
+            a.c.k = a.c.v = ws;
+            a.c.k_scale = a.c.v_scale = (float*)ws;
+        }
         a.blocks = (a.group + S::kHeads - 1) / S::kHeads;
         a.unit_tokens = y.unit_tokens;
         a.start_units = y.start_units;

@@ -438,7 +438,7 @@ chm_status chm_cache_read(const chm_kv_cache* cache, const int64_t* slots, int64
  * with token j of sequence b in page tables[b, j / page_size] and query heads
  * h sharing key head h / (q_heads / cache->heads).
  * q and out: [batch, q_heads, dim] of `type` (token_stride unused): fp16 or
- * bf16, the cache's own type for 16-bit caches.  tables: int32
+ * bf16, the cache's own type for 16-bit caches; out may be q.  tables: int32
  * [batch, table_width], rows table_stride apart; lens: int32 [batch]; starts:
  * int32 [batch] or NULL for zeros (a window: lens - window; below 0 counts as
  * 0); lse: fp32 [batch, q_heads] contiguous, or NULL.

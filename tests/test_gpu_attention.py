@@ -655,6 +655,64 @@ def test_attention_of_nothing():
     assert bool(out.isnan().all() & lse.isnan().all())
 
 
+@pytest.mark.parametrize("held,t,group", [("bf16", None, 7), ("fp16", None, 12), ("int8", "bf16", 4), ("e4m3", "fp16", 1)])
+@pytest.mark.parametrize("lens", [[20011], [1, 9000, 0, 5, 17000]])
+def test_attention_split_over_its_length(lens, held, t, group):
+    """Sequences cut into many parts.  The sums over n tokens add 2 n u of sum p |v| to the bound."""
+    c = Case(lens=lens, q_heads=2 * group, k_heads=2, dim=128, page=16, held=held, t=t, seed=group)
+    got, lse = c.run()
+    out, want, tol, ltol = c.expected()
+    more = 2 * max(lens) * U
+    within(got, out, tol + more * c.values(c.vp, c.vs).abs().amax())
+    within(lse, want, ltol + more)
+    whole = c.tables.clone()
+    worst = max(range(len(lens)), key=lambda i: lens[i])
+    c.tables[worst, lens[worst] // 32] = c.n + 7   # a page in the middle that is not there
+    got2, lse2 = c.run()
+    assert bool(got2[worst].isnan().all() & lse2[worst].isnan().all())
+    c.tables = whole
+    rest = [i for i in range(len(lens)) if i != worst]
+    assert all(torch.equal(got2[i], got[i]) and torch.equal(lse2[i], lse[i]) for i in rest)
+    # one token left of the longest
+    c.s = torch.zeros(len(lens), dtype=torch.int32, device=DEV)
+    c.starts = [0] * len(lens)
+    c.starts[worst] = lens[worst] - 1
+    c.s[worst] = lens[worst] - 1
+    c.check()
+
+
+def test_attention_in_place_and_without_pages():
+    c = Case(lens=[700, 3, 2000], q_heads=16, k_heads=2, dim=64, page=16, held="e4m3", t="bf16")
+    want, _ = c.run()
+    got, _ = c.run(out=c.q)
+    assert got is c.q and torch.equal(got, want)
+    none = c.kp[:0], c.vp[:0]
+    out, lse = A.paged_attention(c.q, *none, c.tables, c.l, c.ks[:0], c.vs[:0])
+    assert bool(out.isnan().all() & lse.isnan().all())
+
+
+def test_graph_of_split_sequences():
+    """Two calls captured back to back on one workspace, replayed as lengths and caches change."""
+    c = Case(lens=[1, 9000, 0, 4000], q_heads=16, k_heads=2, dim=128, page=16, held="bf16")
+    d = Case(lens=[6000, 70, 0, 0], q_heads=16, k_heads=2, dim=128, page=16, held="bf16", seed=1,
+             width=c.tables.shape[1])
+    ws = torch.empty(A.paged_attention_workspace(c.kp, c.vp, 4, 16, c.tables.shape[1]), dtype=torch.uint8, device=DEV)
+    c.run(workspace=ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a, b = c.run(workspace=ws), d.run(workspace=ws)
+    for lens in ([1, 9000, 0, 4000], [0, 17, 0, 4000], [16, 8999, 3000, 1]):
+        c.l.copy_(torch.tensor(lens, device=DEV))
+        c.tables[2] = c.tables[1]   # two sequences may share pages
+        d.q.normal_()
+        ws.fill_(0xFF)
+        graph.replay()
+        got = [x.clone() for x in (*a, *b)]
+        want = [*c.run(), *d.run()]
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 def test_results_do_not_depend_on_the_run():
     c = Case(lens=[1900, 3, 700, 0, 64], q_heads=28, k_heads=4, dim=128, page=16, held="e4m3", t="bf16")
     a = c.run()
