@@ -17,7 +17,9 @@ at most 256.
 
 Every call runs on `stream` (default: the current stream of its tensors'
 device), allocates its outputs there where none are given, never synchronises,
-and can be captured into a CUDA graph.  Arguments that do not fit raise
+and can be captured into a CUDA graph.  As with any work on a stream of one's
+own, its order against the tensors' other uses is the caller's, and so is keeping
+them until it is done (torch.Tensor.record_stream).  Arguments that do not fit raise
 TypeError or ValueError before anything is launched; so do tensors that
 require a gradient while gradients are recorded.
 """

@@ -17,8 +17,12 @@
 //   most warps through the remainder (32,768 tokens of 8 heads of 128 to e4m3: 63 us
 //   against 48).
 //
-// Both directions move their bytes once; the bound is HBM, and next to it the
-// instructions per value (the integer pipe runs at half rate).
+// Both directions move their bytes once; the bound is HBM, and next to it, for
+// codes, the instructions per value (134 per warp and vector of 128 to write, 90 to
+// read; the integer pipe, at half rate, is busy for two thirds of the writing).  One
+// B200: 32,768 tokens of 8 heads of 128 bf16 values written to e4m3 in 47 us (203 MB,
+// 4.3 TB/s) and read back in 35 (5.7 TB/s); 8,192 to a bf16 cache in 12 and back in 12
+// (67 MB each, 5.6 TB/s).
 #include <cuda_fp8.h>
 
 #include <type_traits>

@@ -3,16 +3,29 @@
 //
 // out = sum_j p_j v_j / sum_j p_j with p_j = exp(scale <q, k_j> - m), one pass
 // over the tokens with a running maximum m.  Every key and value is read once,
-// for all the query heads that share it, so the bound is HBM.
+// for all the query heads that share it, so the bound is HBM: 2 G flops per
+// element read for G heads, where the device has time for 500 per bf16 element.
 //
 // The products run on mma.sync m16n8k16 with the tokens (for the scores) and
 // the elements of the value vector (for the output) as the 16 rows and the
 // query heads of one key head as the 8 columns:
 //   S^T [tokens x heads] = K [tokens x dim] Q^T,   O^T [dim x heads] += V^T P^T.
 // Both contractions may take their index in any order, so a thread's 16-byte
-// runs are its operand registers as they come: each lane copies its own runs
-// into a ring of its own in shared memory, steps ahead, and reads them back;
-// no layout to swizzle, no barrier.
+// runs are its operand registers as they come; 8-bit codes become fp16 numbers in
+// registers.  (tcgen05 would take K and V from shared memory only: codes would go
+// there a second time, and values transposed.  At 8 cycles per product the tensor
+// cores are busy for 15 to 25% of the time as it is.)  Each warp copies its runs
+// into a ring of its own in shared memory ahead of their use.
+//
+// One B200, us per call: 64 sequences of up to 4,096 tokens (32 query heads on 8
+// key heads of 128, bf16) 99 for 546 MB, 5.5 TB/s; one sequence of 262,144 tokens
+// (28 on 4 of 128, int8) 62 for 277 MB, 4.4 TB/s; 128 documents of up to 2,000
+// tokens (20 on 4 of 64, e4m3) 37 for 72 MB.  A call that joins parts costs about 11
+// for no tokens at all: two launches, some 3 us from a block's start to its first
+// product, 1 to 2 at each segment's end.  Past that, 16-bit caches stream at 6.5 TB/s;
+// 8-bit ones are bound by the instructions of 10 to 12 warps per SM beside that (0.56
+// issued per cycle; more warps, fewer instructions or shorter chains of products
+// did not change the time).
 #include <algorithm>
 #include <cmath>
 #include <cstdio>
@@ -236,6 +249,7 @@ struct Shape {
     // long sequence 66 us in place of 64.
     static constexpr int kSlot = kTok * DMAX * kBytes;
     static constexpr int kSlots = (kResident == 3 ? 8192 : kResident == 2 ? 16384 : 32768) / kSlot;
+    static_assert(kSlots % 2 == 0, "keys take even slots, values odd ones");
     static constexpr int kScaleSlots = kSlots / 2 + 1;  // steps whose scales are on their way or in use
     // shared memory: q as operand registers, factors of its rows, rings, scales, the warps' parts
     static constexpr int kQ = NT * (DMAX / 32) * 512 + kHeads * 4;
@@ -448,8 +462,8 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) qf[n][e] = kWide ? a.scale_log2 : s_f[n * 8 + 2 * t + e];
 
-            // The copies run kSlots half steps ahead: what has just been read makes room for the
-            // newest step's values or the next one's keys.
+            // The copies run kSlots / 2 steps ahead: keys that have been read make room for those
+            // of the step that far ahead, its values for its values.
             int slot = 0, scale_out = 0;
             for (int base = now.first + warp * kTok; base < now.end; base += kTile) {
                 const uint8_t* const keys = ring + slot * kSlot + lane * 16;
@@ -529,10 +543,7 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
                         for (int e = 0; e < 4; ++e)
                             above = above || (kWide ? sc[n][i][e] : sc[n][i][e] + lv[i][e >> 1]) > m[n][e & 1] + kRoom;
                 __syncwarp();  // all lanes have read the keys and scales
-                if (kSlots % 2)
-                    its_values(slot);
-                else
-                    next_keys(now, slot);
+                next_keys(now, slot);
                 slot = slot + 1 == kSlots ? 0 : slot + 1;
                 // ---- the reference follows the largest exponent
                 if (__any_sync(0xffffffffu, above)) {
@@ -615,10 +626,7 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
                     }
                 }
                 __syncwarp();
-                if (kSlots % 2)
-                    next_keys(now, slot);
-                else
-                    its_values(slot);
+                its_values(slot);
                 slot = slot + 1 == kSlots ? 0 : slot + 1;
             }
             copies_wait<0>();

@@ -548,6 +548,40 @@ def test_attention_with_nan_and_infinite_tokens(held):
     assert torch.equal(got[1, 2:], clean[1, 2:]) and torch.equal(got[2:], clean[2:])
 
 
+def test_attention_over_every_code():
+    """Caches of arbitrary bytes: int8's -128, and e4m3's NaN codes, which make their own NaN and no other."""
+    g = gen(6)
+    for held in ("int8", "e4m3"):
+        ht = NAMES[held]
+        raw = torch.randint(0, 256, (2, 9, 2, 16, 128), generator=g, device=DEV).to(torch.uint8)
+        if held == "e4m3":
+            raw = torch.where((raw & 0x7F) == 0x7F, torch.zeros_like(raw), raw)
+        c = Case(lens=[140], q_heads=4, k_heads=2, dim=128, page=16, held=held, t="bf16", spare=0)
+        c.kp, c.vp = raw[0].clone().view(ht), raw[1].clone().view(ht)
+        c.q = c.q * (0.02 if held == "int8" else 0.05)
+        clean, clse = c.check()
+        if held == "e4m3":
+            c.vp.view(torch.uint8)[c.tables[0, 3], 1, 5, 77] = 0xFF
+            got, lse = c.run()
+            bad = got.isnan()
+            assert bool(bad[0, 2:, 77].all()) and int(bad.sum()) == 2 and torch.equal(lse, clse)
+            c.kp.view(torch.uint8)[c.tables[0, 8], 0, 2, 0] = 0x7F
+            got, lse = c.run()
+            assert bool(got[0, :2].isnan().all() & lse[0, :2].isnan().all()) and torch.equal(lse[0, 2:], clse[0, 2:])
+
+
+def test_attention_of_many_sequences():
+    lens = [(i * 7) % 40 for i in range(5000)]
+    c = Case(lens=lens, q_heads=4, k_heads=1, dim=16, page=16, held="fp16", width=64)
+    got, lse = c.run()
+    few = [0, 1, 2, 127, 128, 129, 2500, 4998, 4999]
+    c.lens = [lens[i] for i in few]
+    c.q, c.tables = c.q[few], c.tables[few]
+    out, want, tol, ltol = c.expected()
+    within(got[few], out, tol)
+    within(lse[few], want, ltol)
+
+
 def test_attention_where_every_score_is_minus_infinity():
     """Infinite keys: all scores -inf gives an empty row, some -inf leave the others."""
     c = Case(lens=[150, 150], q_heads=2, k_heads=1, dim=16, page=16, held="bf16")
