@@ -75,6 +75,7 @@ struct AttArgs {
     int32_t* before;  // units before each sequence
     Boundary* boundaries;
     float* parts;
+    int32_t main_blocks; // of the main kernel
     bool join_segments;  // the join's blocks stand for segments, not boundaries
 };
 
@@ -208,15 +209,75 @@ struct Range {
     bool bad;  // the length does not fit the table
 };
 
-__device__ __forceinline__ Range sequence_range(const AttArgs& a, int b) {
+__device__ __forceinline__ Range range_of(const AttArgs& a, int start, int len) {
     Range r;
-    r.first = a.starts ? min(max(a.starts[b], 0), a.capacity) : 0;
-    r.end = a.lens[b];
+    r.first = min(max(start, 0), a.capacity);
+    r.end = len;
     r.bad = r.end > a.capacity;
     if (r.bad) r.end = 0;
     r.units = a.start_units + max(1, (int)a.by_unit.div((uint32_t)(max(r.end - r.first, 0) + a.unit_tokens - 1)));
     return r;
 }
+__device__ __forceinline__ Range sequence_range(const AttArgs& a, int b) {
+    return range_of(a, a.starts ? a.starts[b] : 0, a.lens[b]);
+}
+
+// Where the units of up to 128 sequences lie, worked out by a warp: lane i has
+// those of sequences i, 32 + i, 64 + i and 96 + i, and the sums up to them.
+struct Deal {
+    int n[4], sum[4];
+    int total;
+
+    __device__ __forceinline__ Deal(const AttArgs& a, int segs, int lane) {
+        int len[4], start[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int i = k * 32 + lane;
+            len[k] = i < a.batch ? a.lens[i] : 0;
+            start[k] = a.starts && i < a.batch ? a.starts[i] : 0;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            sum[k] = n[k] = k * 32 + lane < a.batch ? range_of(a, start[k], len[k]).units * segs : 0;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int y = __shfl_up_sync(0xffffffffu, sum[k], x);
+                if (lane >= x) sum[k] += y;
+            }
+        total = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int all = __shfl_sync(0xffffffffu, sum[k], 31);
+            sum[k] += total;
+            total += all;
+        }
+    }
+    // The sequence that holds unit u < total, and the units before it.
+    __device__ __forceinline__ int find(int u, int& before) const {
+        int b = 0;
+#pragma unroll
+        for (int k = 3; k >= 0; --k) {
+            const uint32_t past = __ballot_sync(0xffffffffu, sum[k] > u);
+            if (past) {
+                const int at = __ffs(past) - 1;
+                b = k * 32 + at;
+                before = __shfl_sync(0xffffffffu, sum[k] - n[k], at);
+            }
+        }
+        return b;
+    }
+    __device__ __forceinline__ int before(int b) const {
+        int y = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int x = __shfl_sync(0xffffffffu, sum[k] - n[k], b & 31);
+            if (b >> 5 == k) y = x;
+        }
+        return y;
+    }
+};
 
 // Rows of parts: DMAX output elements, then the reference and the sum.  Block c
 // has slot 2c for the segment that holds its first unit and 2c + 1 for its last.
@@ -776,9 +837,11 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
     }
 }
 
-// Block (x, h): head h of a segment that several blocks had, from its parts in
-// the order of the blocks.  x stands for a segment or, where there are fewer, for
-// the boundary before block x + 1 (then the segment's first boundary does it).
+// Block (x, y): some heads, a row of threads each, of a segment that several blocks had,
+// from its parts in the order of the blocks.  x stands for a segment or, where there are
+// fewer, for the boundary before block x + 1 (then the segment's first boundary does it).
+// Which parts there are follows from the lengths: up to 128 sequences that is worked out
+// while the main kernel's last blocks run, else read from what the main kernel left.
 constexpr int kJoinThreads = 256;
 
 template <int DMAX, int NT>
@@ -788,28 +851,48 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const AttA
     constexpr int kAhead = kV > 4 ? 4 : 8;  // parts on their way per warp
     __shared__ float s_acc[kJoinThreads / 32][DMAX];
     __shared__ float s_sum[kJoinThreads / 32], s_top[kJoinThreads / 32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const Plan plan = *a.plan;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;  // of this row of threads
     const int segs = a.c.heads * a.blocks;
-    Boundary s;
-    if (a.join_segments) {
-        s.seq = blockIdx.x / segs;
-        s.seg = blockIdx.x - s.seq * segs;
+    const bool early = a.batch <= 128;
+    Plan plan{1, 0};
+    Boundary s{0, 0, 0, 1};
+    bool any = true;
+    if (early) {
+        const Deal deal(a, segs, lane);
+        plan = Plan{(deal.total + a.main_blocks - 1) / a.main_blocks, deal.total};
+        if (a.join_segments) {
+            s.seq = blockIdx.x / segs;
+            s.first = deal.before(s.seq);
+        } else {
+            const int64_t u = (blockIdx.x + 1) * (int64_t)plan.per;
+            any = u < plan.total;
+            if (any) s.seq = deal.find((int)u, s.first);
+        }
         s.units = sequence_range(a, s.seq).units;
-        s.first = a.before[s.seq] + s.seg * s.units;
-    } else {
-        const int64_t u = (blockIdx.x + 1) * (int64_t)plan.per;
-        if (u >= plan.total) return;
-        s = a.boundaries[blockIdx.x + 1];
-        if (s.first == u || s.first / plan.per != (int)blockIdx.x) return;
+        s.seg = a.join_segments ? blockIdx.x - s.seq * segs : ((int)(blockIdx.x + 1) * plan.per - s.first) / s.units;
+        s.first += s.seg * s.units;
     }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!early) {
+        plan = *a.plan;
+        if (a.join_segments) {
+            s.seq = blockIdx.x / segs;
+            s.seg = blockIdx.x - s.seq * segs;
+            s.units = sequence_range(a, s.seq).units;
+            s.first = a.before[s.seq] + s.seg * s.units;
+        } else {
+            any = (blockIdx.x + 1) * (int64_t)plan.per < plan.total;
+            if (any) s = a.boundaries[blockIdx.x + 1];
+        }
+    }
+    if (!any) return;
     const int c0 = s.first / plan.per, c1 = (s.first + s.units - 1) / plan.per;
-    if (c0 == c1) return;
+    // a boundary: one inside the segment, and its first
+    if (c0 == c1 || (!a.join_segments && c0 != (int)blockIdx.x)) return;
     const int head = s.seg / a.blocks;
     const int h0 = head * a.group + (s.seg - head * a.blocks) * kHeads;
-    const int hh = blockIdx.y;
-    if (h0 + hh >= (head + 1) * a.group) return;
+    const int hh = blockIdx.y * blockDim.y + threadIdx.y;
+    if (hh >= kHeads || h0 + hh >= (head + 1) * a.group) return;
     const int odd = c0 * plan.per != s.first;  // whether the first part is its block's second slot
     auto part = [&](int i) { return part_row<DMAX>(a.parts, 2 * i + (i == c0 ? odd : 0), kHeads, hh); };
     // each warp takes every warps-th part, kAhead of them on their way at once
@@ -953,6 +1036,7 @@ struct Launch {
         a.by_unit = FastDiv((uint32_t)y.unit_tokens);
         const int64_t segments = (int64_t)a.batch * y.segs;
         a.join_segments = segments < y.blocks;
+        a.main_blocks = y.blocks;
         static bool set[64];  // per device: the kernel may take this much shared memory
         int dev = 0;
         CHM_CUDA(cudaGetDevice(&dev));
@@ -966,12 +1050,13 @@ struct Launch {
         if (!y.joins || y.blocks < 2) return CHM_OK;
         // The join's blocks start while the main kernel's last ones run, and wait for its end.
         cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3((unsigned)(a.join_segments ? segments : y.blocks - 1), (unsigned)std::min(S::kHeads, a.group));
-        // a warp has 8 parts on their way: warps enough for eight rounds of the most a segment
-        // can have (64 sequences up to 4,096 tokens, 128 long documents: one warp 99.6 and 37.4
-        // us, four 100.0 and 38.1; one sequence of 262,144: eight)
+        // A warp has 8 parts on their way: warps enough for eight rounds of the most a segment
+        // can have, and a row of one warp for each head where one is enough.
         const int64_t most = std::min<int64_t>(y.blocks, y.units / segments);
-        cfg.blockDim = dim3((unsigned)std::min<int64_t>(kJoinThreads, 32 * ((most + 63) / 64)));
+        const int warps = (int)std::min<int64_t>(kJoinThreads / 32, (most + 63) / 64), heads = std::min(S::kHeads, a.group);
+        const int rows = warps == 1 ? std::min(heads, 8) : 1;
+        cfg.gridDim = dim3((unsigned)(a.join_segments ? segments : y.blocks - 1), (unsigned)((heads + rows - 1) / rows));
+        cfg.blockDim = dim3((unsigned)(32 * warps), (unsigned)rows);
         cfg.stream = st;
         cudaLaunchAttribute attr{};
         attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
