@@ -841,7 +841,8 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
 // from its parts in the order of the blocks.  x stands for a segment or, where there are
 // fewer, for the boundary before block x + 1 (then the segment's first boundary does it).
 // Which parts there are follows from the lengths: up to 128 sequences that is worked out
-// while the main kernel's last blocks run, else read from what the main kernel left.
+// while the main kernel's last blocks run (one sequence of 600 tokens 7.7 us against 8.8,
+// 16 of them 12.7 against 13.1), else read from what the main kernel left.
 constexpr int kJoinThreads = 256;
 
 template <int DMAX, int NT>
@@ -981,7 +982,10 @@ struct Launch {
 
     static Layout layout(const AttArgs& a) {
         Layout y;
-        // up to 4 tiles a segment stays whole: a second launch costs more than they do
+        // Up to 4 tiles a segment stays whole: a second launch and the parts cost more than
+        // they do.  One sequence / 32 of them (32 query heads on 8 of 128, bf16, device time):
+        // 2 tiles 6.2 / 7.8 us whole, 7.0 / 12.7 split; 4 tiles 7.7 / 9.7 and 7.1 / 12.7; 8 tiles
+        // 10.9 / 13.6 and 7.6 / 16.4.
         const int whole = 4 * S::kTile;
         y.unit_tokens = a.capacity <= whole ? whole : S::kTile;
         y.joins = a.capacity > whole;
@@ -1070,7 +1074,10 @@ struct Launch {
 
 // Calls f on the Launch<> for a cache's type, dim and sharing.  More than 8
 // query heads per key head take two blocks of 8 at a time, so that up to 16
-// read the cache once; at dim 256 the registers hold one block.
+// read the cache once: 32 sequences of 4,096 tokens, 2 key heads of 128, bf16, 16 /
+// 9 query heads each 35 / 34 us, by single blocks 38 / 37; 128 sequences of 128
+// tokens 13 against 17 (one of 8,192 tokens 14 against 12).  At dim 256 the
+// registers hold one block.
 template <int KIND, typename F>
 static auto with_kind(const AttArgs& a, F f) {
     if (a.c.dim > 128) return f(Launch<256, KIND, 1>{});
