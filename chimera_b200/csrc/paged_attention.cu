@@ -20,7 +20,7 @@
 // One B200, us per call: 64 sequences of up to 4,096 tokens (32 query heads on 8
 // key heads of 128, bf16) 99 for 546 MB, 5.5 TB/s; one sequence of 262,144 tokens
 // (28 on 4 of 128, int8) 62 for 277 MB, 4.4 TB/s; 128 documents of up to 2,000
-// tokens (20 on 4 of 64, e4m3) 37 for 72 MB.  A call that joins parts costs about 11
+// tokens (20 on 4 of 64, e4m3) 37 for 72 MB.  A call that joins parts costs about 10
 // for no tokens at all: two launches, some 3 us from a block's start to its first
 // product, 1 to 2 at each segment's end.  Past that, 16-bit caches stream at 6.5 TB/s;
 // 8-bit ones are bound by the instructions of 10 to 12 warps per SM beside that (0.56
@@ -343,6 +343,10 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
     // weights (their high part) so stay below 2^15, and the smallest step of their low part,
     // 2^-24, is 2^-35 of the largest: many small ones are not lost.  bf16 has fp32's range.
     constexpr float kLead = kHalf ? 11.0f : 0.0f, kRoom = kHalf ? 15.0f : 8.0f;
+    // A value's scale counts as at least 2^-80: without values exp2(score - ref) is then below
+    // 2^95 and its sum over 2^30 tokens finite, and the smallest scale that is written, 2^-105,
+    // still has weights that fp16 holds.
+    constexpr float kLeast = -80.0f;
     extern __shared__ __align__(16) uint8_t smem[];
     uint4(*s_q)[kRuns][32] = reinterpret_cast<uint4(*)[kRuns][32]>(smem);
     float* const s_f = reinterpret_cast<float*>(smem + NT * kRuns * 512);
@@ -561,7 +565,14 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
                             }
                         }
                     }
-                // ---- scaled; tokens past the end get weight zero
+                // ---- scaled, by q's factor first (the keys' alone could overflow); tokens past the
+                // end get weight zero
+#pragma unroll
+                for (int i = 0; i < kU; ++i)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sc[n][i][e] *= qf[n][e & 1];
                 float vs[kU][2], lv[kU][2];
                 if (!kWide) {
 #pragma unroll
@@ -571,7 +582,7 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
                             const int src = i * 16 + h * 8 + g;
                             const float ks = scales[scale_out * 2 * kTok + src];
                             vs[i][h] = scales[scale_out * 2 * kTok + kTok + src];
-                            lv[i][h] = fmaxf(log2_fast(fabsf(vs[i][h])), -105.0f);  // the smallest scale written
+                            lv[i][h] = fmaxf(log2_fast(fabsf(vs[i][h])), kLeast);
 #pragma unroll
                             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -580,12 +591,6 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
                     scale_out = scale_out + 1 == kScaleSlots ? 0 : scale_out + 1;
                 }
                 bool above = false;
-#pragma unroll
-                for (int i = 0; i < kU; ++i)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) sc[n][i][e] *= qf[n][e & 1];
                 if (base + kTok > now.end) {
 #pragma unroll
                     for (int i = 0; i < kU; ++i)

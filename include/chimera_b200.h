@@ -449,12 +449,14 @@ chm_status chm_cache_read(const chm_kv_cache* cache, const int64_t* slots, int64
  * Softmax statistics and sums are fp32; probabilities enter the value product
  * as two 16-bit terms (high and remainder); beside 8-bit caches q enters the
  * score product as fp16, brought into its range by a power of two per row
- * (exact but for elements below 2^-28 of the row's largest).  A sequence may be cut elsewhere in
- * another batch or with a wider table, which moves the rounding of its sums;
- * the same call gives the same bits every time.
+ * (exact but for elements below 2^-28 of the row's largest), and where 8-bit
+ * values pass 2^110 in magnitude, probabilities below 2^-16 of the largest may
+ * count as zero.  A sequence may be cut elsewhere in another batch or with a
+ * wider table, which moves the rounding of its sums; the same call gives the
+ * same bits every time.
  * table_width * page_size is at most 2^30, batch 65,535, and the keys' and the
- * values' memory span at most 64 GB each.  Calls on one
- * workspace must not overlap. */
+ * values' memory span at most 64 GB each.  Calls on one workspace must not
+ * overlap. */
 size_t chm_paged_attention_workspace_bytes(const chm_kv_cache* cache, int64_t batch, int32_t q_heads,
                                            int32_t table_width);
 chm_status chm_paged_attention(const chm_kv_cache* cache, const chm_heads* q, const chm_heads* out, int32_t type,

@@ -23,7 +23,6 @@ relative rounding of fp32 and half_step the one of the output's type
 """
 import math
 
-import numpy as np
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -568,6 +567,40 @@ def test_attention_over_every_code():
             c.kp.view(torch.uint8)[c.tables[0, 8], 0, 2, 0] = 0x7F
             got, lse = c.run()
             assert bool(got[0, :2].isnan().all() & lse[0, :2].isnan().all()) and torch.equal(lse[0, 2:], clse[0, 2:])
+
+
+@pytest.mark.parametrize("held", ["int8", "e4m3"])
+@pytest.mark.parametrize("by", [0.0, 2.0 ** -94, 2.0 ** -60, 2.0 ** 100])
+def test_attention_of_values_of_any_size(held, by):
+    """Values that are all zero, near the smallest that are held, and huge: the weights carry their scale, lse does
+    not.  Below 2^-80 a weight may be held by fp16's 11 bits alone: 2^-11 of sum p |v| more."""
+    c = Case(lens=[3000, 40, 1], q_heads=6, k_heads=2, dim=64, page=16, held=held, t="bf16")
+    flat = torch.randn(c.n * 16, 2, 64, generator=gen(7), device=DEV)
+    slots = torch.arange(c.n * 16, device=DEV)
+    k, _ = A.cache_read(slots, c.kp, c.vp, c.ks, c.vs, dtype=torch.float32)
+    A.cache_write(k, flat * by, slots, c.kp, c.vp, c.ks, c.vs)
+    got, lse = c.run()
+    c.vs = c.vs.double() / (by or 1.0)     # the same values of ordinary size, in 64 bits
+    out, want, tol, ltol = c.expected()
+    within(lse, want, ltol)
+    assert bool(lse.isfinite().all())
+    room = tol + (2.0 ** -11 * 5 if by < 2.0 ** -80 else 0)
+    within(got.double() / (by or 1.0), out, room)
+
+
+@pytest.mark.parametrize("held,t", [("int8", "bf16"), ("e4m3", "bf16"), ("bf16", None)])
+@pytest.mark.parametrize("up", [90, -90])
+def test_attention_of_queries_and_keys_far_from_one(held, t, up):
+    """Queries by 2^-up and keys by 2^up: powers of two, so the scores are the same."""
+    c = Case(lens=[1000, 40], q_heads=6, k_heads=2, dim=64, page=16, held=held, t=t)
+    want, wlse = c.run()
+    c.q = c.q * 2.0 ** -up
+    if c.ks is None:
+        c.kp *= 2.0 ** up
+    else:
+        c.ks *= 2.0 ** up
+    got, lse = c.run()
+    assert torch.equal(got, want) and torch.equal(lse, wlse)
 
 
 def test_attention_of_many_sequences():
