@@ -32,10 +32,15 @@
 namespace chm {
 
 constexpr int kCacheThreads = 128;
-// Vectors per thread and side.  32,768 tokens of 8 heads of 128 bf16 values to e4m3 and back:
-// 80 us; with 1 for writing 82, 3 for reading 82, 2 for reading 84, 6 for reading 88; 256 threads
-// 2 to 7 more.
+// Vectors per thread and side: one, until there are so many vectors that more loads on their
+// way count for more than more warps.  Device time of one against several:
+//   writing (2): 32 tokens of 8 heads of 128 bf16 values 1.9 / 2.3 us, 8,192 to e4m3 11.8 / 12.0,
+//     32,768 to e4m3 49 / 47;
+//   reading (4): 1.8 / 2.6, 2,048 from e4m3 3.7 / 4.1, 8,192 8.6 / 8.5, 32,768 40 / 35.
+// (32,768 written and read back: 80 us; 1 and 4: 82, 2 and 3: 82, 2 and 2: 84, 256 threads: 2 to
+// 7 more.)
 constexpr int kWriteUnroll = 2, kReadUnroll = 4;
+constexpr int64_t kWriteMany = 131072, kReadMany = 65536;
 
 struct CacheArgs {
     chm_kv_cache c;
@@ -189,16 +194,16 @@ __device__ __forceinline__ Place place_of(const CacheArgs& a, int64_t slot, uint
 }
 
 // A group of LPV lanes holds a vector, 8 elements a lane.
-template <typename T, int KIND, int LPV>
+template <typename T, int KIND, int LPV, int U>
 __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const CacheArgs a) {
     constexpr int kPer = kCacheThreads / LPV;
     const int lane = threadIdx.x % LPV;
-    const int64_t first = (int64_t)blockIdx.x * (kPer * kWriteUnroll) + threadIdx.x / LPV;
-    Eight<T> x[kWriteUnroll][2];
-    Place place[kWriteUnroll];
-    bool on[kWriteUnroll];
+    const int64_t first = (int64_t)blockIdx.x * (kPer * U) + threadIdx.x / LPV;
+    Eight<T> x[U][2];
+    Place place[U];
+    bool on[U];
 #pragma unroll
-    for (int j = 0; j < kWriteUnroll; ++j) {
+    for (int j = 0; j < U; ++j) {
         const int64_t vec = first + j * kPer;
         on[j] = vec < a.vectors;
         const uint32_t t = on[j] ? a.by_heads.div((uint32_t)vec) : 0u;
@@ -216,7 +221,7 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const CacheA
         }
     }
 #pragma unroll
-    for (int j = 0; j < kWriteUnroll; ++j) {
+    for (int j = 0; j < U; ++j) {
         float largest[2];
         if (KIND == CHM_INT8 || KIND == CHM_E4M3) {
             uint32_t top[2] = {x[j][0].top(), x[j][1].top()};
@@ -319,20 +324,20 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const CacheA
     }
 }
 
-template <typename T, int KIND, int LPV>
+template <typename T, int KIND, int LPV, int U>
 __global__ void __launch_bounds__(kCacheThreads) cache_read_kernel(const CacheArgs a) {
     constexpr int kPer = kCacheThreads / LPV;
     constexpr bool kCodes = KIND == CHM_INT8 || KIND == CHM_E4M3;
     using H = typename std::conditional<KIND == CHM_FP16, __half, __nv_bfloat16>::type;
     const int lane = threadIdx.x % LPV;
-    const int64_t first = (int64_t)blockIdx.x * (kPer * kReadUnroll) + threadIdx.x / LPV;
+    const int64_t first = (int64_t)blockIdx.x * (kPer * U) + threadIdx.x / LPV;
     if (lane * 8 >= a.c.dim) return;
-    Eight<H> held[kReadUnroll][2];
-    uint2 codes[kReadUnroll][2];
-    float scale[kReadUnroll][2];
-    uint32_t t[kReadUnroll], h[kReadUnroll];
+    Eight<H> held[U][2];
+    uint2 codes[U][2];
+    float scale[U][2];
+    uint32_t t[U], h[U];
 #pragma unroll
-    for (int j = 0; j < kReadUnroll; ++j) {
+    for (int j = 0; j < U; ++j) {
         const int64_t vec = first + j * kPer;
         t[j] = vec < a.vectors ? a.by_heads.div((uint32_t)vec) : 0u;
         h[j] = (uint32_t)vec - t[j] * a.c.heads;
@@ -355,7 +360,7 @@ __global__ void __launch_bounds__(kCacheThreads) cache_read_kernel(const CacheAr
         }
     }
 #pragma unroll
-    for (int j = 0; j < kReadUnroll; ++j) {
+    for (int j = 0; j < U; ++j) {
         if (first + j * kPer >= a.vectors) continue;
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
@@ -385,24 +390,33 @@ __global__ void __launch_bounds__(kCacheThreads) cache_read_kernel(const CacheAr
     }
 }
 
+template <typename T, int KIND, int LPV, bool WRITE>
+static void launch_lanes(const CacheArgs& a, cudaStream_t st) {
+    constexpr int kMany = WRITE ? kWriteUnroll : kReadUnroll;
+    const bool many = a.vectors >= (WRITE ? kWriteMany : kReadMany);
+    const int per = kCacheThreads / LPV * (many ? kMany : 1);
+    const unsigned grid = (unsigned)((a.vectors + per - 1) / per);
+    if constexpr (WRITE) {
+        if (many)
+            cache_write_kernel<T, KIND, LPV, kMany><<<grid, kCacheThreads, 0, st>>>(a);
+        else
+            cache_write_kernel<T, KIND, LPV, 1><<<grid, kCacheThreads, 0, st>>>(a);
+    } else {
+        if (many)
+            cache_read_kernel<T, KIND, LPV, kMany><<<grid, kCacheThreads, 0, st>>>(a);
+        else
+            cache_read_kernel<T, KIND, LPV, 1><<<grid, kCacheThreads, 0, st>>>(a);
+    }
+}
+
 template <typename T, int KIND, bool WRITE>
 static void launch_cache(const CacheArgs& a, cudaStream_t st) {
-    const int lpv = a.c.dim <= 64 ? 8 : a.c.dim <= 128 ? 16 : 32;
-    const int per = kCacheThreads / lpv * (WRITE ? kWriteUnroll : kReadUnroll);
-    const unsigned grid = (unsigned)((a.vectors + per - 1) / per);
-#define CHM_CACHE_GO(L)                                                      \
-    if (WRITE)                                                               \
-        cache_write_kernel<T, KIND, L><<<grid, kCacheThreads, 0, st>>>(a);   \
-    else                                                                     \
-        cache_read_kernel<T, KIND, L><<<grid, kCacheThreads, 0, st>>>(a)
-    if (lpv == 8) {
-        CHM_CACHE_GO(8);
-    } else if (lpv == 16) {
-        CHM_CACHE_GO(16);
-    } else {
-        CHM_CACHE_GO(32);
-    }
-#undef CHM_CACHE_GO
+    if (a.c.dim <= 64)
+        launch_lanes<T, KIND, 8, WRITE>(a, st);
+    else if (a.c.dim <= 128)
+        launch_lanes<T, KIND, 16, WRITE>(a, st);
+    else
+        launch_lanes<T, KIND, 32, WRITE>(a, st);
 }
 
 template <typename T, bool WRITE>

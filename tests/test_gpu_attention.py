@@ -265,6 +265,30 @@ def test_cache_write_and_read(dim, heads, page, t, held, token_major):
             assert bool((got[~on] == 0).all())
 
 
+@pytest.mark.parametrize("held", ["int8", "e4m3", "bf16"])
+@pytest.mark.parametrize("t", ["fp32", "bf16"])
+@pytest.mark.parametrize("tokens,heads", [(8191, 8), (8192, 8), (16383, 8), (16384, 8), (131073, 1), (43691, 3)])
+def test_cache_of_many_vectors(tokens, heads, t, held):
+    """Counts on both sides of where the kernels take several vectors per thread, and not multiples of them."""
+    ht, dim, page = NAMES[held], 32, 16
+    g = gen(tokens)
+    n = -(-tokens // page)
+    kp, vp, ks, vs = make_pages(n, heads, page, dim, ht)
+    x = torch.randn(2, tokens, heads, dim, generator=g, device=DEV).to(NAMES[t])
+    slots = torch.randperm(n * page, generator=g, device=DEV)[:tokens]
+    slots[-3] = -1
+    A.cache_write(x[0], x[1], slots, kp, vp, ks, vs)
+    k, v = A.cache_read(slots, kp, vp, ks, vs, dtype=torch.float32)
+    for xi, got in ((x[0], k), (x[1], v)):
+        if ht in TOP:
+            code, scale = quantised64(xi, ht)
+            want = code.float() * scale[..., None]
+        else:
+            want = xi.to(ht).float()
+        want[-3] = 0
+        assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("held", ["int8", "e4m3"])
 def test_cache_codes_at_ties_and_neighbours(held):
     """Quotients on, just above and just below the middle between two codes: scale 1 and scales that are not
