@@ -987,15 +987,17 @@ struct Launch {
 
     static Layout layout(const AttArgs& a) {
         Layout y;
-        // Up to 4 tiles a segment stays whole: a second launch and the parts cost more than
-        // they do.  One sequence / 32 of them (32 query heads on 8 of 128, bf16, device time):
-        // 2 tiles 6.2 / 7.8 us whole, 7.0 / 12.7 split; 4 tiles 7.7 / 9.7 and 7.1 / 12.7; 8 tiles
-        // 10.9 / 13.6 and 7.6 / 16.4.
-        const int whole = 4 * S::kTile;
+        y.segs = a.c.heads * ((a.group + S::kHeads - 1) / S::kHeads);
+        // Up to 4 tiles, or 8 where there are segments enough for the device, a segment stays
+        // whole: a second launch and the parts cost more than the balance gains.  Device time
+        // of 1 / 16 / 64 / 128 sequences (32 query heads on 8 of 128, bf16): 2 tiles 6.2 / 6.3 /
+        // 14 / 20 us whole, 7.0 / 10.4 / 16 / 23 split; 4 tiles 7.7 / 8.1 / 19 / 31 and 7.1 / 10.3 /
+        // 18 / 33; 8 tiles 11.0 / 11.2 / 32 / 52 and 7.6 / 12.4 / 31 / 52, of 32 and 48 sequences
+        // 13.6 and 17.4 whole, 16.5 and 21.8 split.
+        const int whole = ((int64_t)a.batch * y.segs >= 128 ? 8 : 4) * S::kTile;
         y.unit_tokens = a.capacity <= whole ? whole : S::kTile;
         y.joins = a.capacity > whole;
         y.start_units = y.joins ? kStartUnits : 0;  // else a segment is one unit
-        y.segs = a.c.heads * ((a.group + S::kHeads - 1) / S::kHeads);
         y.units = (int64_t)a.batch * y.segs * (y.start_units + std::max(1, (a.capacity + y.unit_tokens - 1) / y.unit_tokens));
         y.blocks = (int)std::min<int64_t>(y.units, (int64_t)sm_count() * S::kResident);
         return y;

@@ -772,6 +772,16 @@ def test_attention_split_over_its_length(lens, held, t, group):
     c.check()
 
 
+@pytest.mark.parametrize("held,t", [("bf16", None), ("int8", "bf16")])
+@pytest.mark.parametrize("batch", [1, 63, 64])
+@pytest.mark.parametrize("tokens", [128, 144, 256, 272, 512, 528, 1024, 1040])
+def test_attention_where_segments_begin_to_split(tokens, batch, held, t):
+    """Tables on both sides of the sizes up to which a sequence stays whole, with many heads and sequences and few."""
+    g = torch.Generator().manual_seed(tokens + batch)
+    lens = [tokens] + torch.randint(0, tokens + 1, (batch - 1,), generator=g).tolist()
+    Case(lens=lens, q_heads=6, k_heads=2, dim=64, page=16, held=held, t=t, seed=batch, width=tokens // 16).check()
+
+
 def test_attention_in_place_and_without_pages():
     c = Case(lens=[700, 3, 2000], q_heads=16, k_heads=2, dim=64, page=16, held="e4m3", t="bf16")
     want, _ = c.run()
