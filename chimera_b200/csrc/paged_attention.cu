@@ -212,7 +212,7 @@ struct Range {
 __device__ __forceinline__ Range range_of(const AttArgs& a, int start, int len) {
     Range r;
     r.first = min(max(start, 0), a.capacity);
-    r.end = len;
+    r.end = max(len, 0);  // so that end - first stays within 32 bits
     r.bad = r.end > a.capacity;
     if (r.bad) r.end = 0;
     r.units = a.start_units + max(1, (int)a.by_unit.div((uint32_t)(max(r.end - r.first, 0) + a.unit_tokens - 1)));
