@@ -294,6 +294,38 @@ __device__ __forceinline__ void store_row(const AttArgs& a, int b, int head, int
         static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
 }
 
+// Element d of the output over tokens [first, end) where the products came out NaN beside
+// a finite sum of probabilities.  An infinite value makes them so: the low term of its weight
+// may be 0 or negative, and a weight that 16 bits do not hold is 0.  The probability itself is
+// positive, so with infinities of one sign among the values the element is that infinity; with
+// both, or a NaN, it is NaN.
+template <int KIND>
+__device__ __noinline__ float infinite_element(const AttArgs& a, int b, int head, int first, int end, int d) {
+    bool plus = false, minus = false;
+    for (int j = first; j < end; ++j) {
+        const uint32_t turn = a.by_page.div((uint32_t)j), within = (uint32_t)j - turn * (uint32_t)a.c.page_size;
+        const int64_t page = a.tables[b * a.table_stride + turn];
+        if (page < 0 || page >= a.c.num_pages) return __int_as_float(0x7FC00000);
+        const int64_t at = page * a.c.page_stride + head * a.c.head_stride + within * a.c.token_stride + d;
+        float y;
+        if (KIND == CHM_FP16)
+            y = __half2float(static_cast<const __half*>(a.c.v)[at]);
+        else if (KIND == CHM_BF16)
+            y = __bfloat162float(static_cast<const __nv_bfloat16*>(a.c.v)[at]);
+        else {
+            if (KIND == CHM_INT8)
+                y = (float)static_cast<const int8_t*>(a.c.v)[at];
+            else
+                y = __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t*>(a.c.v)[at], __NV_E4M3)));
+            y *= a.c.v_scale[(page * a.c.heads + head) * a.c.page_size + within];
+        }
+        if (y != y) return y;
+        plus = plus || y == INFINITY;
+        minus = minus || y == -INFINITY;
+    }
+    return plus == minus ? __int_as_float(0x7FC00000) : plus ? INFINITY : -INFINITY;
+}
+
 // DMAX: dim rounded up to 64, 128 or 256; NT: blocks of 8 query heads.
 template <int DMAX, int KIND, int NT>
 struct Shape {
@@ -324,7 +356,7 @@ struct Shape {
 
 template <int DMAX, int KIND, int NT>
 __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
-    paged_attention_kernel(const AttArgs a) {
+    paged_attention_kernel(const __grid_constant__ AttArgs a) {
     using S = Shape<DMAX, KIND, NT>;
     constexpr bool kWide = S::kWide;
     constexpr bool kHalf = KIND != CHM_BF16;  // fp16 products; 8-bit codes are fp16 numbers
@@ -345,7 +377,8 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
     constexpr float kLead = kHalf ? 11.0f : 0.0f, kRoom = kHalf ? 15.0f : 8.0f;
     // A value's scale counts as at least 2^-80: without values exp2(score - ref) is then below
     // 2^95 and its sum over 2^30 tokens finite, and the smallest scale that is written, 2^-105,
-    // still has weights that fp16 holds.
+    // still has weights that fp16 holds.  So does an infinite one: its products are infinite
+    // whatever the reference, which would take the others' probabilities with it.
     constexpr float kLeast = -80.0f;
     extern __shared__ __align__(16) uint8_t smem[];
     uint4(*s_q)[kRuns][32] = reinterpret_cast<uint4(*)[kRuns][32]>(smem);
@@ -582,7 +615,8 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
                             const int src = i * 16 + h * 8 + g;
                             const float ks = scales[scale_out * 2 * kTok + src];
                             vs[i][h] = scales[scale_out * 2 * kTok + kTok + src];
-                            lv[i][h] = fmaxf(log2_fast(fabsf(vs[i][h])), kLeast);
+                            const float x = log2_fast(fabsf(vs[i][h]));
+                            lv[i][h] = x < INFINITY ? fmaxf(x, kLeast) : kLeast;
 #pragma unroll
                             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -769,14 +803,29 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
                 }
                 if (bad) sum = __int_as_float(0x7FC00000);
                 float* part = part_row<DMAX>(a.parts, 2 * blockIdx.x + (piece > 0), kHeads, hh);
-                for (int d = lane; d < dim; d += 32) {
-                    float acc = 0.0f;
+                float acc[DMAX / 32];
+                bool odd = false;
 #pragma unroll
-                    for (int w = 0; w < kAttWarps; ++w) acc += f[w] * s_o[w][hh][d];
+                for (int v = 0; v < DMAX / 32; ++v) {
+                    acc[v] = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < kAttWarps; ++w) acc[v] += f[w] * s_o[w][hh][v * 32 + lane];
+                    odd = odd || acc[v] != acc[v];
+                }
+                if (__any_sync(0xffffffffu, odd) && sum == sum) {
+#pragma unroll
+                    for (int v = 0; v < DMAX / 32; ++v)
+                        if (acc[v] != acc[v] && v * 32 + lane < dim)
+                            acc[v] = infinite_element<KIND>(a, now.b, now.head, now.first, now.end, v * 32 + lane);
+                }
+#pragma unroll
+                for (int v = 0; v < DMAX / 32; ++v) {
+                    const int d = v * 32 + lane;
+                    if (d >= dim) continue;
                     if (now.whole)
-                        store_row(a, now.b, now.h0 + hh, d, sum == 0.0f ? 0.0f : bad ? sum : acc / sum);
+                        store_row(a, now.b, now.h0 + hh, d, sum == 0.0f ? 0.0f : bad ? sum : acc[v] / sum);
                     else
-                        part[d] = acc;
+                        part[d] = acc[v];
                 }
                 if (lane == 0) {
                     if (!now.whole)
@@ -950,9 +999,21 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const AttA
         top = all;
     }
 #pragma unroll
-    for (int v = 0; v < kV; ++v)
-        if (v * 32 + lane < a.c.dim)
-            store_row(a, s.seq, h0 + hh, v * 32 + lane, sum == 0.0f ? 0.0f : sum != sum ? sum : acc[v] / sum);
+    for (int v = 0; v < kV; ++v) {
+        const int d = v * 32 + lane;
+        if (d >= a.c.dim) continue;
+        if (acc[v] != acc[v] && sum == sum) {  // an infinite part, its factor 0 maybe: as infinite_element
+            bool plus = false, minus = false, none = false;
+            for (int i = c0; i <= c1; ++i) {
+                const float y = part(i)[d];
+                plus = plus || y == INFINITY;
+                minus = minus || y == -INFINITY;
+                none = none || y != y;
+            }
+            if (!none && plus != minus) acc[v] = plus ? INFINITY : -INFINITY;
+        }
+        store_row(a, s.seq, h0 + hh, d, sum == 0.0f ? 0.0f : sum != sum ? sum : acc[v] / sum);
+    }
     if (lane == 0 && a.lse)
         a.lse[(int64_t)s.seq * a.q_heads + h0 + hh] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }

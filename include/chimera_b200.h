@@ -446,6 +446,8 @@ chm_status chm_cache_read(const chm_kv_cache* cache, const int64_t* slots, int64
  * -infinity, gets zeros and lse = -infinity.  Pages and parts of pages outside
  * the range are not read.  A page id outside the cache that the range needs,
  * or a length past the table's end, makes the sequence's rows and lse NaN.
+ * An element with infinite values of one sign among those attended to is that
+ * infinity; with both signs, or a NaN, it is NaN.
  * Softmax statistics and sums are fp32; probabilities enter the value product
  * as two 16-bit terms (high and remainder); beside 8-bit caches q enters the
  * score product as fp16, brought into its range by a power of two per row

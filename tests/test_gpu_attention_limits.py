@@ -7,7 +7,8 @@ import pytest
 pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
-from tests.test_gpu_attention import DEV, Case  # noqa: E402
+from chimera_b200 import attention as A  # noqa: E402
+from tests.test_gpu_attention import DEV, Case, within  # noqa: E402
 
 
 I32 = torch.iinfo(torch.int32)
@@ -37,3 +38,87 @@ def test_one_sequence_of_no_length_with_a_start(length, start):
         c = Case(lens=[length], starts=[start], q_heads=4, k_heads=2, dim=64, page=16, held="fp16", width=width)
         got, lse = c.run()
         assert bool((got == 0).all() & (lse == -math.inf).all())
+
+
+def place(c, b, token):
+    return int(c.tables[b, token // c.page]), token % c.page
+
+
+@pytest.mark.parametrize("held", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim,group", [(64, 4), (64, 12), (128, 3), (128, 9), (256, 2), (80, 1)])
+@pytest.mark.parametrize("n", [90, 9000])   # one block, and parts that are joined
+def test_infinite_values(n, dim, group, held):
+    """An element with infinite values of one sign among those attended to is that infinity, with both signs or a
+    NaN it is NaN; all else keeps its bits.  Weights reach from the largest to far below what 16 bits hold."""
+    c = Case(lens=[n, 70], q_heads=2 * group, k_heads=2, dim=dim, page=16, held=held, seed=dim + n)
+    c.q *= 0.5
+    k = c.values(c.kp, None)[c.tables[0].long()].transpose(0, 1).flatten(1, 2)[:, :n]
+    s = torch.einsum("hd,hnd->hn", c.q[0].double(), k.repeat_interleave(group, 0)) * c.scale
+    order = s[0].argsort().tolist()   # by the first row's weights
+    near, far, last = order[-1], order[0], order[n // 2]
+    p, w = place(c, 0, far)
+    c.kp[p, 0, w] *= 16.0             # far below the others for that row, above them for some
+    clean, clse = c.run()
+    inf = math.inf
+    #       element: (token, value), ...
+    marks = {0: [(near, inf)], 1: [(near, -inf)], 2: [(far, inf)], 3: [(far, -inf)], 4: [(last, inf), (near, inf)],
+             5: [(last, inf), (far, -inf)], 6: [(near, inf), (far, math.nan)], 7: [(0, inf)], 8: [(n - 1, -inf)],
+             dim - 1: [(n // 3, inf), (n - 2, inf)], dim - 2: [(n // 3, inf), (n - 2, -inf)]}
+    want = {0: inf, 1: -inf, 2: inf, 3: -inf, 4: inf, 5: math.nan, 6: math.nan, 7: inf, 8: -inf, dim - 1: inf,
+            dim - 2: math.nan}
+    for d, m in marks.items():
+        for token, value in m:
+            p, w = place(c, 0, token)
+            c.vp[p, 0, w, d] = value
+    got, lse = c.run()
+    assert torch.equal(lse, clse)
+    expected = clean.clone()
+    for d, y in want.items():
+        expected[0, :group, d] = y
+    same = (got == expected) | (got.isnan() & expected.isnan())
+    assert bool(same.all()), f"elements {sorted(set((~same).nonzero()[:, 2].tolist()))} differ"
+
+
+@pytest.mark.parametrize("held", ["bf16", "fp16"])
+def test_infinite_values_outside_the_range_change_nothing(held):
+    c = Case(lens=[100, 3000], starts=[20, 1000], q_heads=8, k_heads=2, dim=64, page=16, held=held)
+    clean = c.run()
+    for b, tokens in ((0, (0, 19, 100)), (1, (0, 999, 3000))):
+        for token in tokens:
+            p, w = place(c, b, token)
+            c.vp[p, :, w] = math.inf
+    got = c.run()
+    assert all(torch.equal(x, y) for x, y in zip(got, clean))
+
+
+def test_a_value_past_fp16_is_an_infinity():
+    """cache_write rounds fp32 values above 65,504 to infinities in an fp16 cache."""
+    c = Case(lens=[300], q_heads=4, k_heads=2, dim=64, page=16, held="fp16")
+    _, clse = c.run()
+    slots = torch.tensor([int(c.tables[0, 8]) * 16 + 5], device=DEV)
+    k, v = A.cache_read(slots, c.kp, c.vp, dtype=torch.float32)
+    v[0, 1, 7], v[0, 1, 9] = 1e5, -1e5
+    A.cache_write(k, v, slots, c.kp, c.vp)
+    got, lse = c.run()
+    assert torch.equal(lse, clse)
+    assert bool((got[0, 2:, 7] == math.inf).all() & (got[0, 2:, 9] == -math.inf).all())
+    got[0, 2:, 7] = got[0, 2:, 9] = 0
+    assert bool(got.isfinite().all())
+
+
+@pytest.mark.parametrize("held", ["int8", "e4m3"])
+@pytest.mark.parametrize("n", [200, 9000])
+def test_infinite_scales_of_values(n, held):
+    """Values are code * scale: infinities by the codes' signs, NaN where a code is 0; lse does not see them."""
+    c = Case(lens=[n, 70], q_heads=6, k_heads=2, dim=64, page=16, held=held, t="bf16", seed=n)
+    clean, _ = c.run()
+    _, sums, _, tol = c.expected()
+    p, w = place(c, 0, n // 2)
+    c.vp.view(torch.uint8)[p, 1, w, 5] = 0
+    c.vs[p, 1, w] = math.inf
+    code = c.vp[p, 1, w].float()
+    got, lse = c.run()
+    within(lse, sums, tol + 2 * n * 2.0 ** -24)
+    want = clean.clone()
+    want[0, 3:] = code * math.inf
+    assert bool(((got == want) | (got.isnan() & want.isnan())).all())
