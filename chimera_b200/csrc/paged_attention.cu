@@ -378,7 +378,9 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
     // A value's scale counts as at least 2^-80: without values exp2(score - ref) is then below
     // 2^95 and its sum over 2^30 tokens finite, and the smallest scale that is written, 2^-105,
     // still has weights that fp16 holds.  So does an infinite one: its products are infinite
-    // whatever the reference, which would take the others' probabilities with it.
+    // whatever the reference, which would take the others' probabilities with it.  References
+    // may so differ by 200 beside sums of up to 2^95: a sum takes the factor between two of
+    // them, which may be below 2^-126, in two halves.
     constexpr float kLeast = -80.0f;
     extern __shared__ __align__(16) uint8_t smem[];
     uint4(*s_q)[kRuns][32] = reinterpret_cast<uint4(*)[kRuns][32]>(smem);
@@ -660,9 +662,9 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
 #pragma unroll
                             for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
                             top -= kLead;
-                            const float f = top > m[n][e] ? exp2_fast(m[n][e] - top) : 1.0f;
+                            const float half = top > m[n][e] ? exp2_fast(0.5f * (m[n][e] - top)) : 1.0f, f = half * half;
                             m[n][e] = fmaxf(top, m[n][e]);
-                            l[n][e] *= f;
+                            l[n][e] = l[n][e] * half * half;
 #pragma unroll
                             for (int i = 0; i < kM; ++i) o[n][i][e] *= f, o[n][i][2 + e] *= f;
                         }
@@ -798,8 +800,9 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
                 for (int w = 0; w < kAttWarps; ++w) top = fmaxf(top, s_m[w][hh]);
 #pragma unroll
                 for (int w = 0; w < kAttWarps; ++w) {
-                    f[w] = s_m[w][hh] == -INFINITY ? 0.0f : exp2_fast(s_m[w][hh] - top);
-                    sum += f[w] * s_l[w][hh];
+                    const float half = s_m[w][hh] == -INFINITY ? 0.0f : exp2_fast(0.5f * (s_m[w][hh] - top));
+                    f[w] = half * half;
+                    sum += s_l[w][hh] * half * half;
                 }
                 if (bad) sum = __int_as_float(0x7FC00000);
                 float* part = part_row<DMAX>(a.parts, 2 * blockIdx.x + (piece > 0), kHeads, hh);
@@ -966,15 +969,15 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const AttA
         float now = top;
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) now = fmaxf(now, m[j]);
-        const float f = top == now ? 1.0f : exp2_fast(top - now);
+        const float half = top == now ? 1.0f : exp2_fast(0.5f * (top - now)), f = half * half;
         top = now;
-        sum *= f;
+        sum = sum * half * half;
 #pragma unroll
         for (int v = 0; v < kV; ++v) acc[v] *= f;
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
-            const float w = m[j] == -INFINITY ? 0.0f : exp2_fast(m[j] - top);
-            sum += l[j] * w;
+            const float half = m[j] == -INFINITY ? 0.0f : exp2_fast(0.5f * (m[j] - top)), w = half * half;
+            sum += l[j] * half * half;
 #pragma unroll
             for (int v = 0; v < kV; ++v) acc[v] += x[j][v] * w;
         }
@@ -991,8 +994,8 @@ __global__ void __launch_bounds__(kJoinThreads) attention_join_kernel(const AttA
 #pragma unroll
         for (int v = 0; v < kV; ++v) acc[v] = 0.0f;
         for (int w = 0; w < warps; ++w) {
-            const float f = s_top[w] == -INFINITY ? 0.0f : exp2_fast(s_top[w] - all);
-            sum += f * s_sum[w];
+            const float half = s_top[w] == -INFINITY ? 0.0f : exp2_fast(0.5f * (s_top[w] - all)), f = half * half;
+            sum += s_sum[w] * half * half;
 #pragma unroll
             for (int v = 0; v < kV; ++v) acc[v] += f * s_acc[w][v * 32 + lane];
         }

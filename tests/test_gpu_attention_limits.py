@@ -8,7 +8,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 from chimera_b200 import attention as A  # noqa: E402
-from tests.test_gpu_attention import DEV, Case, within  # noqa: E402
+from tests.test_gpu_attention import DEV, Case, gen, within  # noqa: E402
 
 
 I32 = torch.iinfo(torch.int32)
@@ -122,3 +122,35 @@ def test_infinite_scales_of_values(n, held):
     want = clean.clone()
     want[0, 3:] = code * math.inf
     assert bool(((got == want) | (got.isnan() & want.isnan())).all())
+
+
+@pytest.mark.parametrize("held", ["int8", "e4m3"])
+@pytest.mark.parametrize("by", [2.0 ** 50, 2.0 ** 60, 2.0 ** 100])
+@pytest.mark.parametrize("zero", [
+    lambda j, n: j < n // 2,             # all of the first warps, steps, blocks
+    lambda j, n: j >= n // 2,
+    lambda j, n: j % 2 == 0,             # within every step
+    lambda j, n: j // 32 % 2 == 0,       # warp by warp
+    lambda j, n: j // 128 % 2 == 0,      # step by step
+    lambda j, n: j != n - 1,             # one token has values, the last
+    lambda j, n: j != 0,
+])
+@pytest.mark.parametrize("n", [64, 500, 9000])
+def test_sums_beside_scales_far_apart(n, zero, by, held):
+    """Vectors of zeros beside huge ones, scores alike or a few units apart: the sum of the probabilities keeps those
+    of both, though the exponents that the weights are taken against differ by up to 180."""
+    c = Case(lens=[n], q_heads=4, k_heads=2, dim=64, page=16, held=held, t="bf16", seed=n, spare=0)
+    slots = c.tables[0].long().repeat_interleave(16) * 16 + torch.arange(16, device=DEV).repeat(c.tables.shape[1])
+    k, v = A.cache_read(slots, c.kp, c.vp, c.ks, c.vs, dtype=torch.float32)
+    v = torch.randn(v.shape, generator=gen(3), device=DEV).clamp(-3, 3) * by
+    v[zero(torch.arange(len(slots), device=DEV), n)] = 0
+    A.cache_write(k, v, slots, c.kp, c.vp, c.ks, c.vs)
+    for spread in (0.0, 1.0):
+        c.q.normal_(generator=gen(4)).mul_(spread)
+        got, lse = c.run()
+        held_vs, c.vs = c.vs, c.vs.double() / by
+        out, want, tol, ltol = c.expected()
+        c.vs = held_vs
+        more = 2 * n * 2.0 ** -24
+        within(lse, want, ltol + more)
+        within(got.double() / by, out, tol + more * 3)
