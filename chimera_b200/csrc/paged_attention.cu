@@ -344,8 +344,8 @@ struct Shape {
     static constexpr int kSlots = (kResident == 3 ? 8192 : kResident == 2 ? 16384 : 32768) / kSlot;
     static_assert(kSlots % 2 == 0, "keys take even slots, values odd ones");
     static constexpr int kScaleSlots = kSlots / 2 + 1;  // steps whose scales are on their way or in use
-    // shared memory: q as operand registers, factors of its rows, rings, scales, the warps' parts
-    static constexpr int kQ = NT * (DMAX / 32) * 512 + kHeads * 4;
+    // shared memory: q as operand registers, two factors of its rows, rings, scales, the warps' parts
+    static constexpr int kQ = NT * (DMAX / 32) * 512 + kHeads * 8;
     static constexpr int kRing = kAttWarps * kSlots * kSlot;
     static constexpr int kScales = kWide ? 0 : kAttWarps * kScaleSlots * 2 * kTok * 4;
     static constexpr int kRow = DMAX + 4;
@@ -556,11 +556,14 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
 #pragma unroll
         for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.0f;
         if (piece >= 0) {
-            float qf[NT][2];
+            float qf[NT][2], qg[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) qf[n][e] = kWide ? a.scale_log2 : s_f[n * 8 + 2 * t + e];
+                for (int e = 0; e < 2; ++e) {
+                    qf[n][e] = kWide ? a.scale_log2 : s_f[n * 8 + 2 * t + e];
+                    qg[n][e] = kWide ? 1.0f : s_f[kHeads + n * 8 + 2 * t + e];
+                }
 
             // The copies run kSlots / 2 steps ahead: keys that have been read make room for those
             // of the step that far ahead, its values for its values.
@@ -600,8 +603,8 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
                             }
                         }
                     }
-                // ---- scaled, by q's factor first (the keys' alone could overflow); tokens past the
-                // end get weight zero
+                // ---- scaled: by half of q's factor, the key's scale, the other half, so that neither
+                // passes fp32's range where the score does not; tokens past the end get weight zero
 #pragma unroll
                 for (int i = 0; i < kU; ++i)
 #pragma unroll
@@ -622,7 +625,7 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
 #pragma unroll
                             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                                for (int e = 0; e < 2; ++e) sc[n][i][h * 2 + e] *= ks;
+                                for (int e = 0; e < 2; ++e) sc[n][i][h * 2 + e] = sc[n][i][h * 2 + e] * ks * qg[n][e];
                         }
                     scale_out = scale_out + 1 == kScaleSlots ? 0 : scale_out + 1;
                 }
@@ -867,25 +870,28 @@ __global__ void __launch_bounds__(kAttThreads, Shape<DMAX, KIND, NT>::kResident)
                         x[2 * e] = y.x, x[2 * e + 1] = y.y;
                     }
                 }
-                float up = 1.0f, f = a.scale_log2;
+                float f = a.scale_log2, f2 = 1.0f;
                 if (!kWide) {
                     float top = 0.0f;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) top = isfinite(x[e]) ? fmaxf(top, fabsf(x[e])) : top;
 #pragma unroll
                     for (int y = kLanes / 2; y > 0; y >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, y));
-                    const int e = top > 0.0f ? min(13 - ilogbf(top), 100) : 0;
-                    up = exp2f((float)e);
-                    f *= exp2f((float)-e);
+                    const int y = top > 0.0f ? 13 - ilogbf(top) : 0;  // -114 to 146: in two halves
+                    const float up = exp2f((float)(y / 2)), up2 = exp2f((float)(y - y / 2));
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = x[e] * up * up2;
+                    f *= exp2f((float)-(y / 2));
+                    f2 = exp2f((float)-(y - y / 2));
                 }
                 uint32_t w[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = pack16<kHalf>(x[2 * e] * up, x[2 * e + 1] * up);
+                for (int e = 0; e < 4; ++e) w[e] = pack16<kHalf>(x[2 * e], x[2 * e + 1]);
                 const int run = kWide ? d0 / 32 : d0 / 64 * 2 + (d0 / 8) % 2;
                 const int tt = kWide ? d0 / 8 % 4 : d0 / 16 % 4;
                 if (hh < kHeads) {
                     s_q[hh / 8][run][hh % 8 * 4 + tt] = make_uint4(w[0], w[1], w[2], w[3]);
-                    if (d0 == 0) s_f[hh] = f;
+                    if (d0 == 0) s_f[hh] = f, s_f[kHeads + hh] = f2;
                 }
             }
         }

@@ -154,3 +154,18 @@ def test_sums_beside_scales_far_apart(n, zero, by, held):
         more = 2 * n * 2.0 ** -24
         within(lse, want, ltol + more)
         within(got.double() / by, out, tol + more * 3)
+
+
+@pytest.mark.parametrize("held", ["int8", "e4m3"])
+@pytest.mark.parametrize("up", [126, 100, 60, -60, -100, -116])
+def test_queries_from_the_ends_of_bf16(held, up):
+    """Whole numbers by 2^-up as queries, keys by 2^up: powers of two, exact in every place, so the scores and all
+    that follows keep their bits."""
+    c = Case(lens=[1000, 40], q_heads=6, k_heads=2, dim=64, page=16, held=held, t="bf16")
+    c.q = torch.randint(-100, 101, c.q.shape, generator=gen(1), device=DEV).bfloat16()
+    want, wlse = c.run(scale=0.004)
+    c.q = c.q * 2.0 ** -up
+    c.ks *= 2.0 ** up
+    assert bool(c.ks.isfinite().all() & (c.ks >= 2.0 ** -126).logical_or(c.ks == 0).all())
+    got, lse = c.run(scale=0.004)
+    assert torch.equal(got, want) and torch.equal(lse, wlse)
