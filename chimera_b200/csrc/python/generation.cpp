@@ -83,6 +83,15 @@ Tensor output(PyObject* o, c10::IntArrayRef shape, ScalarType type, c10::Device 
     return x;
 }
 
+// Tells autograd that a caller's tensor was written (one it saved is then refused by
+// backward).  Tensors of inference mode have no count, and cannot be saved.
+void written(const Tensor& x) {
+    if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+}
+void written(PyObject* o) {
+    if (o != Py_None) written(THPVariable_Unpack(o));
+}
+
 bool flag(PyObject* o) {
     const int r = PyObject_IsTrue(o);
     if (r < 0) throw python_error();
@@ -167,6 +176,8 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
                      pos.data_ptr(), (int32_t)pos.element_size(), per_row ? pos.stride(0) : 0,
                      pos.stride(per_row ? 1 : 0), freqs.data_ptr<double>(), scale, flags, stream_of(dev)),
           "rotary");
+    written(a[7]);
+    written(a[8]);
     PyObject* r0 = a[7] != Py_None ? Py_NewRef(a[7]) : THPVariable_Wrap(qo);
     PyObject* r1 = !both ? Py_NewRef(Py_None) : a[8] != Py_None ? Py_NewRef(a[8]) : THPVariable_Wrap(ko);
     return pair(r0, r1);
@@ -236,6 +247,7 @@ PyObject* cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const chm_heads kh = heads_of(k, "k", false, true), vh = heads_of(v, "v", false, true);
     const c10::cuda::CUDAGuard guard(dev);
     check(chm_cache_write(&c, &kh, &vh, type, slots.size(0), slots.data_ptr<int64_t>(), stream_of(dev)), "cache_write");
+    for (int i = 3; i < 7; ++i) written(a[i]);
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }
@@ -256,6 +268,8 @@ PyObject* cache_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor k = output(a[6], shape, st, dev, "k_out"), v = output(a[7], shape, st, dev, "v_out");
     const chm_heads kh = heads_of(k, "k_out", false, true), vh = heads_of(v, "v_out", false, true);
     check(chm_cache_read(&c, slots.data_ptr<int64_t>(), slots.size(0), &kh, &vh, type, stream_of(dev)), "cache_read");
+    written(a[6]);
+    written(a[7]);
     PyObject* r0 = a[6] != Py_None ? Py_NewRef(a[6]) : THPVariable_Wrap(k);
     PyObject* r1 = a[7] != Py_None ? Py_NewRef(a[7]) : THPVariable_Wrap(v);
     return pair(r0, r1);
@@ -313,6 +327,9 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
                               bounds[1], scale, lse.data_ptr<float>(), ws, ws_bytes,
                               stream_of(dev)),
           "paged_attention");
+    written(a[9]);
+    written(a[10]);
+    written(a[11]);
     PyObject* r0 = a[9] != Py_None ? Py_NewRef(a[9]) : THPVariable_Wrap(out);
     PyObject* r1 = a[10] != Py_None ? Py_NewRef(a[10]) : THPVariable_Wrap(lse);
     return pair(r0, r1);

@@ -1,0 +1,71 @@
+"""The generation operators as calls on torch tensors, on the GPU: what autograd
+sees of them, and which tensors are taken and refused."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+from chimera_b200 import attention as A  # noqa: E402
+from tests.test_gpu_attention import DEV, Case, make_pages  # noqa: E402
+
+
+def versions(*xs):
+    return [x._version for x in xs]
+
+
+def test_what_is_written_counts_as_changed():
+    """Tensors that a call writes have their version raised, those it reads not."""
+    f = A.rotary_frequencies(64, device=DEV)
+    pos = torch.arange(5, device=DEV)
+    q, k, qo, ko = (torch.randn(5, 2, 64, device=DEV).bfloat16() for _ in range(4))
+    before = versions(q, k, qo, ko)
+    A.rotary(q, k, pos, f)
+    assert versions(q, k, qo, ko) == before
+    A.rotary(q, k, pos, f, q_out=qo, k_out=ko)
+    after = versions(q, k, qo, ko)
+    assert after[:2] == before[:2] and after[2] > before[2] and after[3] > before[3]
+    A.rotary(q, None, pos, f, q_out=q)
+    assert q._version > before[0] and k._version == before[1]
+
+    for held in (torch.int8, torch.bfloat16):
+        cache = make_pages(2, 2, 8, 64, held)
+        there = [x for x in cache if x is not None]
+        before = versions(k, *there)
+        A.cache_write(k, k, pos, *cache)
+        after = versions(k, *there)
+        assert after[0] == before[0] and all(a > b for a, b in zip(after[1:], before[1:]))
+        A.cache_read(pos, *cache, k_out=ko, v_out=qo)
+        assert versions(k, *there) == after
+
+    c = Case(lens=[40, 9], q_heads=4, k_heads=2, dim=64, page=16, held="int8", t="bf16")
+    out, lse = c.run()
+    there = [c.q, c.kp, c.vp, c.ks, c.vs, c.tables, c.l]
+    before, seen = versions(*there), versions(out, lse)
+    c.run(out=out, lse=lse)
+    assert versions(*there) == before and all(a > b for a, b in zip(versions(out, lse), seen))
+
+
+def test_a_saved_tensor_that_is_turned_in_place_is_noticed():
+    f = A.rotary_frequencies(64, device=DEV)
+    pos = torch.arange(5, device=DEV)
+    w = torch.randn(5, 2, 64, device=DEV, requires_grad=True)
+    x = torch.randn(5, 2, 64, device=DEV)
+    y = (w * x).sum()     # saves x
+    with torch.no_grad():
+        A.rotary(x, None, pos, f, q_out=x)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_tensors_of_inference_mode_are_taken_everywhere():
+    f = A.rotary_frequencies(64, device=DEV)
+    pos = torch.arange(5, device=DEV)
+    with torch.inference_mode():
+        x = torch.randn(5, 2, 64, device=DEV)
+        cache = make_pages(2, 2, 8, 64, torch.int8)
+        A.rotary(x, None, pos, f, q_out=x)
+        A.cache_write(x, x, pos, *cache)
+    A.rotary(x, None, pos, f, q_out=x)
+    A.cache_write(x, x, pos, *cache)
+    k, v = A.cache_read(pos, *cache, dtype=torch.float32)
+    assert torch.equal(k, v)
