@@ -21,8 +21,9 @@ and can be captured into a CUDA graph.  As with any work on a stream of one's
 own, its order against the tensors' other uses is the caller's, and so is keeping
 them until it is done (torch.Tensor.record_stream).  Arguments that do not fit raise
 TypeError or ValueError before anything is launched; so do tensors that
-require a gradient while gradients are recorded.  Tensors that a call writes
-(outputs given to it, pages, scales) count as modified in place.
+require a gradient while gradients are recorded, and tensors with a
+forward-mode tangent.  Tensors that a call writes (outputs given to it, pages,
+scales) count as modified in place.
 """
 from __future__ import annotations
 

@@ -11,6 +11,7 @@
 #include <ATen/Functions.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -48,6 +49,9 @@ const Tensor& tensor(PyObject* o, const char* name) {
     TORCH_CHECK_VALUE(!(x.requires_grad() && at::GradMode::is_enabled()), name,
                       " requires a gradient, which this call does not record: detach it, or call under "
                       "torch.no_grad() (rotary's gradient is rotary with inverse=True)");
+    TORCH_CHECK_VALUE(!(c10::AutogradState::get_tls_state().get_fw_grad_mode() && x._fw_grad(0).defined()), name,
+                      " has a forward-mode tangent, which this call does not carry on: take its primal "
+                      "(torch.autograd.forward_ad.unpack_dual)");
     return x;
 }
 

@@ -69,3 +69,26 @@ def test_tensors_of_inference_mode_are_taken_everywhere():
     A.cache_write(x, x, pos, *cache)
     k, v = A.cache_read(pos, *cache, dtype=torch.float32)
     assert torch.equal(k, v)
+
+
+def test_tensors_with_tangents_are_refused():
+    """A call that would drop a forward-mode tangent says so, under no_grad too."""
+    import torch.autograd.forward_ad as ad
+    f = A.rotary_frequencies(64, device=DEV)
+    c = Case(lens=[40, 9], q_heads=4, k_heads=2, dim=64, page=16, held="bf16")
+    pos = torch.arange(2, device=DEV)
+    with ad.dual_level():
+        q = ad.make_dual(c.q, torch.ones_like(c.q))
+        k = q[:, :2]
+        assert ad.unpack_dual(k).tangent is not None
+        for call in (lambda: A.rotary(q, None, pos, f), lambda: A.rotary(c.q, k, pos, f),
+                     lambda: A.cache_write(k, c.q[:, :2], pos, c.kp, c.vp),
+                     lambda: A.cache_write(c.q[:, :2], k, pos, c.kp, c.vp),
+                     lambda: A.paged_attention(q, c.kp, c.vp, c.tables, c.l)):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
+                call()
+        A.rotary(c.q, None, pos, f)     # tensors without one are taken
+        c.run()
+        A.rotary(ad.unpack_dual(q).primal, None, pos, f)
