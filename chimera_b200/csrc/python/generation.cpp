@@ -195,8 +195,13 @@ chm_kv_cache cache_of(PyObject* const* a, c10::Device dev) {
     const int type = type_of(k.scalar_type());
     TORCH_CHECK_TYPE(type > CHM_FP32, "pages must be float16, bfloat16, int8 or float8_e4m3fn");
     TORCH_CHECK_VALUE(k.dim() == 4, "pages must be [num_pages, heads, page_size, dim]");
-    TORCH_CHECK_VALUE(v.scalar_type() == k.scalar_type() && v.sizes() == k.sizes() && v.strides() == k.strides(),
-                      "k_pages and v_pages must be alike in type, shape and strides");
+    bool alike = v.scalar_type() == k.scalar_type() && v.sizes() == k.sizes();
+    int64_t stride[3] = {};  // of an axis of one any stride will do
+    for (int i = 0; alike && i < 4; ++i) {
+        alike = k.size(i) <= 1 || v.stride(i) == k.stride(i);
+        if (i < 3 && k.size(i) > 1) stride[i] = k.stride(i);
+    }
+    TORCH_CHECK_VALUE(alike, "k_pages and v_pages must be alike in type, shape and strides");
     TORCH_CHECK_VALUE(k.stride(3) == 1 || k.size(3) <= 1, "the last axis of the pages must be contiguous");
     TORCH_CHECK_VALUE(k.size(1) <= (1 << 16) && k.size(2) <= INT32_MAX && k.size(3) <= 256,
                       "pages have at most 65536 heads, 2^31 - 1 tokens and 256 dimensions");
@@ -207,9 +212,9 @@ chm_kv_cache cache_of(PyObject* const* a, c10::Device dev) {
     c.heads = (int32_t)k.size(1);
     c.page_size = (int32_t)k.size(2);
     c.dim = (int32_t)k.size(3);
-    c.page_stride = k.stride(0);
-    c.head_stride = k.stride(1);
-    c.token_stride = k.stride(2);
+    c.page_stride = stride[0];
+    c.head_stride = stride[1];
+    c.token_stride = stride[2];
     c.type = type;
     if (type == CHM_INT8 || type == CHM_E4M3) {
         for (int i = 0; i < 2; ++i) {

@@ -92,3 +92,34 @@ def test_tensors_with_tangents_are_refused():
         A.rotary(c.q, None, pos, f)     # tensors without one are taken
         c.run()
         A.rotary(ad.unpack_dual(q).primal, None, pos, f)
+
+
+@pytest.mark.parametrize("held", ["bf16", "int8"])
+def test_strides_of_axes_of_one_do_not_matter(held):
+    """k and v pages of one page, one head or one token a page, as views with any stride along that axis."""
+    for pages, heads, page in ((1, 2, 16), (5, 1, 16), (3, 2, 1), (1, 1, 1)):
+        n = min(pages * page, 9)
+        c = Case(lens=[n], q_heads=2 * heads, k_heads=heads, dim=64, page=page, held=held, t="bf16",
+                 spare=pages - -(-n // page))
+        want, wlse = c.run()
+
+        def restrided(x, by):
+            s = [by if x.shape[i] == 1 else x.stride(i) for i in range(3)] + [1]
+            return x.as_strided(x.shape, s, x.storage_offset())
+        c.vp = restrided(c.vp, 7)
+        got, lse = c.run()
+        assert torch.equal(got, want) and torch.equal(lse, wlse)
+        c.kp = restrided(c.kp, 1 << 40)
+        got, lse = c.run()
+        assert torch.equal(got, want) and torch.equal(lse, wlse)
+        slots = torch.arange(c.n * page, device=DEV)
+        k, v = A.cache_read(slots, c.kp, c.vp, c.ks, c.vs)
+        A.cache_write(k, v, slots, c.kp, c.vp, c.ks, c.vs)
+        plain = make_pages(c.n, heads, page, 64, c.ht)
+        A.cache_write(k, v, slots, *plain)
+        for x, y in zip(A.cache_read(slots, c.kp, c.vp, c.ks, c.vs), A.cache_read(slots, *plain)):
+            assert torch.equal(x, y)
+    # where an axis has more than one, k and v still go alike
+    c = Case(lens=[9], q_heads=4, k_heads=2, dim=64, page=16, held=held, t="bf16")
+    with pytest.raises(ValueError):
+        A.paged_attention(c.q, c.kp, c.vp.transpose(1, 2).contiguous().transpose(1, 2), c.tables, c.l, c.ks, c.vs)
