@@ -23,7 +23,8 @@ them until it is done (torch.Tensor.record_stream).  Arguments that do not fit r
 TypeError or ValueError before anything is launched; so do tensors that
 require a gradient while gradients are recorded, and tensors with a
 forward-mode tangent.  Tensors that a call writes (outputs given to it, pages,
-scales) count as modified in place.
+scales) count as modified in place; one whose vectors share memory (an expanded
+one), or that starts where another one does, is refused.
 """
 from __future__ import annotations
 

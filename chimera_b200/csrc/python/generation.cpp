@@ -77,6 +77,32 @@ chm_heads heads_of(const Tensor& x, const char* name, bool batch, bool token) {
     return h;
 }
 
+// Whether vectors of x may share memory: an axis, from the smallest stride up, that does not
+// step past all that the ones before it span.
+bool overlaps_itself(const Tensor& x) {
+    const int64_t n = x.dim();
+    if (x.numel() == 0) return false;
+    int64_t extent = x.size(n - 1), done_axes = 0;
+    for (int64_t done = 0; done < n - 1; ++done) {
+        int64_t best = -1;  // the smallest stride of an axis of more than one that is not done
+        for (int64_t i = 0; i < n - 1; ++i)
+            if (x.size(i) > 1 && !(done_axes >> i & 1) && (best < 0 || x.stride(i) < x.stride(best))) best = i;
+        if (best < 0) break;
+        if (x.stride(best) < extent) return true;
+        extent += x.stride(best) * (x.size(best) - 1);
+        done_axes |= int64_t{1} << best;
+    }
+    return false;
+}
+// What a call writes must not overlap itself, nor two outputs stand in one place.
+void check_written(const Tensor& x, const char* name) {
+    TORCH_CHECK_VALUE(!overlaps_itself(x), name, " is written and must not overlap itself");
+}
+void check_apart(const Tensor& x, const Tensor& y, const char* names) {
+    TORCH_CHECK_VALUE(x.numel() == 0 || y.numel() == 0 || x.data_ptr() != y.data_ptr(), names,
+                      " are written and must not overlap");
+}
+
 // An output given by the caller, or a new one.
 Tensor output(PyObject* o, c10::IntArrayRef shape, ScalarType type, c10::Device device, const char* name) {
     // (not at::empty: its dispatch is a third of a small call)
@@ -84,6 +110,7 @@ Tensor output(PyObject* o, c10::IntArrayRef shape, ScalarType type, c10::Device 
     const Tensor& x = tensor_on(device, o, name);
     TORCH_CHECK_VALUE(x.sizes() == shape && x.scalar_type() == type, name, " must be ", c10::toString(type),
                       " of shape ", shape);
+    check_written(x, name);
     return x;
 }
 
@@ -175,6 +202,7 @@ PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
         ko = output(a[8], k->sizes(), k->scalar_type(), dev, "k_out");
         in[1] = heads_of(*k, "k", dims == 4, true);
         out[1] = heads_of(ko, "k_out", dims == 4, true);
+        check_apart(qo, ko, "q_out and k_out");
     }
     check(chm_rotary(in, out, both ? 2 : 1, type, batch, tokens, (int32_t)dim, 2 * (int32_t)freqs.size(0),
                      pos.data_ptr(), (int32_t)pos.element_size(), per_row ? pos.stride(0) : 0,
@@ -254,6 +282,10 @@ PyObject* cache_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
                           v.sizes() == k.sizes(),
                       "k and v must be [", slots.size(0), ", ", c.heads, ", ", c.dim, "]");
     const chm_heads kh = heads_of(k, "k", false, true), vh = heads_of(v, "v", false, true);
+    const Tensor &kp = THPVariable_Unpack(a[3]), &vp = THPVariable_Unpack(a[4]);
+    check_written(kp, "k_pages");  // v_pages has the same strides
+    check_apart(kp, vp, "k_pages and v_pages");
+    if (c.k_scale) check_apart(THPVariable_Unpack(a[5]), THPVariable_Unpack(a[6]), "k_scale and v_scale");
     const c10::cuda::CUDAGuard guard(dev);
     check(chm_cache_write(&c, &kh, &vh, type, slots.size(0), slots.data_ptr<int64_t>(), stream_of(dev)), "cache_write");
     for (int i = 3; i < 7; ++i) written(a[i]);
@@ -276,6 +308,7 @@ PyObject* cache_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const c10::cuda::CUDAGuard guard(dev);
     const Tensor k = output(a[6], shape, st, dev, "k_out"), v = output(a[7], shape, st, dev, "v_out");
     const chm_heads kh = heads_of(k, "k_out", false, true), vh = heads_of(v, "v_out", false, true);
+    check_apart(k, v, "k_out and v_out");
     check(chm_cache_read(&c, slots.data_ptr<int64_t>(), slots.size(0), &kh, &vh, type, stream_of(dev)), "cache_read");
     written(a[6]);
     written(a[7]);

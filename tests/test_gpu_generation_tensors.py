@@ -123,3 +123,37 @@ def test_strides_of_axes_of_one_do_not_matter(held):
     c = Case(lens=[9], q_heads=4, k_heads=2, dim=64, page=16, held=held, t="bf16")
     with pytest.raises(ValueError):
         A.paged_attention(c.q, c.kp, c.vp.transpose(1, 2).contiguous().transpose(1, 2), c.tables, c.l, c.ks, c.vs)
+
+
+def test_outputs_that_overlap_are_refused():
+    f = A.rotary_frequencies(64, device=DEV)
+    c = Case(lens=[40, 9], q_heads=4, k_heads=2, dim=64, page=16, held="int8", t="bf16")
+    pos = torch.arange(2, device=DEV)
+    kv = c.q[:, :2].contiguous()
+    one = torch.zeros(1, 1, 64, dtype=torch.bfloat16, device=DEV)
+    lines = torch.zeros(4 * 64, dtype=torch.bfloat16, device=DEV).as_strided((2, 2, 64), (64, 32, 1))
+    wide = make_pages(1, 2, 16, 64, torch.int8)
+    over = [x.expand(3, *x.shape[1:]) for x in wide[:2]]
+    scales = [torch.zeros(3, 2, 16, device=DEV) for _ in range(2)]
+    for call in (lambda: A.rotary(c.q, None, pos, f, q_out=one.expand(2, 4, 64)),
+                 lambda: A.rotary(kv, kv, pos, f, k_out=one.expand(2, 2, 64)),
+                 lambda: A.rotary(kv, None, pos, f, q_out=lines),
+                 lambda: A.rotary(one.expand(2, 4, 64), None, pos, f, q_out=one.expand(2, 4, 64)),
+                 lambda: A.cache_read(pos, c.kp, c.vp, c.ks, c.vs, k_out=one.expand(2, 2, 64)),
+                 lambda: A.cache_read(pos, c.kp, c.vp, c.ks, c.vs, v_out=lines),
+                 lambda: A.cache_write(kv, kv, pos, *over, *scales),
+                 lambda: c.run(out=one.expand(2, 4, 64)),
+                 lambda: A.rotary(kv, kv, pos, f, q_out=kv, k_out=kv),     # or one another
+                 lambda: A.cache_read(pos, c.kp, c.vp, c.ks, c.vs, k_out=kv, v_out=kv),
+                 lambda: A.cache_write(kv, kv, pos, c.kp, c.kp, c.ks, c.vs),
+                 lambda: A.cache_write(kv, kv, pos, c.kp, c.vp, c.ks, c.ks)):
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+    # read, they may: a page that stands three times, keys that are the values too, heads that share one vector
+    A.cache_read(pos, *over, *scales)
+    A.cache_read(pos, c.kp, c.kp, c.ks, c.ks)
+    A.paged_attention(c.q, c.kp, c.kp, c.tables, c.l, c.ks, c.ks)
+    A.rotary(one.expand(2, 4, 64), None, pos, f)
+    # axes of one, and outputs with their axes in another order, do not overlap
+    A.rotary(one, None, pos[:1], f, q_out=torch.zeros(64, dtype=torch.bfloat16, device=DEV).as_strided((1, 1, 64), (0, 0, 1)))
+    A.rotary(c.q, None, pos, f, q_out=torch.zeros(4, 2, 64, dtype=torch.bfloat16, device=DEV).transpose(0, 1))
