@@ -1093,17 +1093,22 @@ struct Launch {
             a->parts = (float*)parts;
         }
     }
+    // Units are counted in 32 bits.
+    static bool too_much(const Layout& y) {
+        if (y.units <= INT32_MAX - (1 << 20)) return false;
+        set_last_message("paged_attention: too much work for one call");
+        return true;
+    }
     static size_t workspace(const AttArgs& a) {
+        const Layout y = layout(a);
+        if (too_much(y)) return 0;
         Counter c;
-        carve(c, layout(a), nullptr, a.batch);
+        carve(c, y, nullptr, a.batch);
         return c.s.off;
     }
     static chm_status run(AttArgs a, void* ws, size_t ws_bytes, cudaStream_t st) {
         const Layout y = layout(a);
-        if (y.units > INT32_MAX - (1 << 20)) {  // units are counted in 32 bits
-            set_last_message("paged_attention: too much work for one call");
-            return CHM_ERR_INVALID;
-        }
+        if (too_much(y)) return CHM_ERR_INVALID;
         Arena arena(ws, ws_bytes);
         carve(arena, y, &a, a.batch);
         if (arena.overflow) return CHM_ERR_CAPACITY;
@@ -1187,15 +1192,25 @@ static chm_status refuse_attention(const char* why) {
     return CHM_ERR_INVALID;
 }
 
+// What is wrong with a call's sizes, or NULL.
+static const char* bad_sizes(const chm_kv_cache& c, int64_t batch, int32_t q_heads, int32_t table_width) {
+    if (batch < 0 || table_width < 0) return "negative size";
+    if (q_heads < 1 || q_heads % c.heads) return "query heads must be a multiple of the cache's heads";
+    if (batch > 65535) return "at most 65535 sequences";
+    if ((int64_t)table_width * c.page_size > (1 << 30)) return "a table spans at most 2^30 tokens";
+    return nullptr;
+}
+
 }  // namespace chm
 
 extern "C" size_t chm_paged_attention_workspace_bytes(const chm_kv_cache* cache, int64_t batch, int32_t q_heads,
                                                       int32_t table_width) {
     using namespace chm;
     if (check_cache(cache, "paged_attention") != CHM_OK) return 0;
-    if (batch < 0 || batch > 65535 || q_heads < 1 || q_heads % cache->heads || table_width < 0 ||
-        (int64_t)table_width * cache->page_size > (1 << 30))
+    if (const char* why = bad_sizes(*cache, batch, q_heads, table_width)) {
+        refuse_attention(why);
         return 0;
+    }
     AttArgs a{};
     a.c = *cache;
     a.batch = (int32_t)batch;
@@ -1215,11 +1230,8 @@ extern "C" chm_status chm_paged_attention(const chm_kv_cache* cache, const chm_h
     if (type != CHM_FP16 && type != CHM_BF16) return refuse_attention("queries are fp16 or bf16");
     if (type_bytes(cache->type) == 2 && cache->type != type)
         return refuse_attention("queries have the type of a 16-bit cache");
-    if (batch < 0 || table_width < 0) return refuse_attention("negative size");
-    if (q->heads < 1 || q->heads != out->heads || q->heads % cache->heads)
-        return refuse_attention("query heads must be a multiple of the cache's heads");
-    if (batch > 65535) return refuse_attention("at most 65535 sequences");
-    if ((int64_t)table_width * cache->page_size > (1 << 30)) return refuse_attention("a table spans at most 2^30 tokens");
+    if (const char* why = bad_sizes(*cache, batch, q->heads, table_width)) return refuse_attention(why);
+    if (q->heads != out->heads) return refuse_attention("query heads of q and out must agree, a multiple of the cache's heads");
     if (batch == 0) return CHM_OK;
     if (!q->data || !out->data || !lens || (table_width > 0 && !tables)) return refuse_attention("null pointer");
     if (!spans_64gb(*cache)) return refuse_attention("keys and values span at most 64 GB each");

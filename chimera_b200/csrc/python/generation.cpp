@@ -391,7 +391,9 @@ PyObject* paged_attention_workspace(PyObject*, PyObject* const* a, Py_ssize_t n)
         TORCH_CHECK_VALUE(v[i] >= 0 && v[i] <= INT32_MAX, "sizes must be from 0 to 2^31 - 1");
     }
     const c10::cuda::CUDAGuard guard(dev);
-    return PyLong_FromSize_t(chm_paged_attention_workspace_bytes(&c, v[0], (int32_t)v[1], (int32_t)v[2]));
+    const size_t need = chm_paged_attention_workspace_bytes(&c, v[0], (int32_t)v[1], (int32_t)v[2]);
+    TORCH_CHECK_VALUE(need > 0, chm_last_error());
+    return PyLong_FromSize_t(need);
     END_HANDLE_TH_ERRORS
 }
 

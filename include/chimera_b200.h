@@ -458,7 +458,8 @@ chm_status chm_cache_read(const chm_kv_cache* cache, const int64_t* slots, int64
  * same bits every time.
  * table_width * page_size is at most 2^30, batch 65,535, and the keys' and the
  * values' memory span at most 64 GB each.  Calls on one workspace must not
- * overlap. */
+ * overlap.  The workspace of sizes that a call refuses is 0 bytes, the reason in
+ * chm_last_error. */
 size_t chm_paged_attention_workspace_bytes(const chm_kv_cache* cache, int64_t batch, int32_t q_heads,
                                            int32_t table_width);
 chm_status chm_paged_attention(const chm_kv_cache* cache, const chm_heads* q, const chm_heads* out, int32_t type,

@@ -183,3 +183,15 @@ def test_python_calls_want_cuda_tensors():
         A.cache_read(i, pages, pages)
     with pytest.raises(TypeError):
         A.paged_attention(x, pages, pages, i, i)
+
+
+@pytest.mark.parametrize("batch,q_heads,width", [(1, 12, 4), (1, 0, 4), (-1, 32, 4), (65536, 32, 4), (1, 32, -1),
+                                                 (1, 32, 1 << 27), (65535, 32, 1 << 26)])
+def test_the_workspace_of_what_is_refused_is_nothing(batch, q_heads, width):
+    """And the reason is the call's; the last has more work than one call takes."""
+    c = cache()
+    assert L.chm_paged_attention_workspace_bytes(C.byref(c), batch, q_heads, width) == 0
+    reason = L.chm_last_error().decode()
+    assert reason.startswith("paged_attention: ")
+    assert attend(c, batch=batch, q_heads=q_heads, width=width, tables=P) == capi.CHM_ERR_INVALID
+    assert L.chm_last_error().decode() == reason

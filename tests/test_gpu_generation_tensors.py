@@ -157,3 +157,12 @@ def test_outputs_that_overlap_are_refused():
     # axes of one, and outputs with their axes in another order, do not overlap
     A.rotary(one, None, pos[:1], f, q_out=torch.zeros(64, dtype=torch.bfloat16, device=DEV).as_strided((1, 1, 64), (0, 0, 1)))
     A.rotary(c.q, None, pos, f, q_out=torch.zeros(4, 2, 64, dtype=torch.bfloat16, device=DEV).transpose(0, 1))
+
+
+def test_the_workspace_of_what_is_refused_is_refused():
+    c = Case(lens=[40, 9], q_heads=4, k_heads=2, dim=64, page=16, held="int8", t="bf16")
+    cache = c.kp, c.vp
+    assert A.paged_attention_workspace(*cache, 2, 4, 3, c.ks, c.vs) > 0
+    for batch, heads, width in ((2, 5, 3), (2, 0, 3), (65536, 4, 3), (2, 4, 1 << 27), (65535, 4, 1 << 26)):
+        with pytest.raises(ValueError):
+            A.paged_attention_workspace(*cache, batch, heads, width, c.ks, c.vs)
