@@ -135,13 +135,23 @@ def build_host(verbose=False):
 
 
 def build_generation():
-    """The operators of chimera_b200/attention.py over torch tensors."""
-    import torch
+    """The operators of chimera_b200/attention.py over torch tensors, for the
+    torch that is installed (whose version stands beside the object files); none
+    without one."""
+    try:
+        import torch
+    except ModuleNotFoundError as e:
+        if e.name != "torch":
+            raise
+        print("torch is not installed: the generation operators over torch tensors are not built")
+        return None
     from torch.utils.cpp_extension import include_paths
     ext = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
     mod = os.path.join(HERE, "_generation" + ext)
     src = os.path.join(CSRC, "python", "generation.cpp")
-    if _stale(mod, [src, os.path.join(INCLUDE, "chimera_b200.h")]):
+    stamp = os.path.join(OBJ, "generation.torch")
+    built_for = open(stamp).read() if os.path.exists(stamp) else None
+    if built_for != str(torch.__version__) or _stale(mod, [src, os.path.join(INCLUDE, "chimera_b200.h")]):
         tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
         inc = ["-isystem" + d for d in include_paths()] + ["-I" + INCLUDE, "-I" + os.path.join(CUDA_HOME, "include"),
                                                           "-I" + sysconfig.get_paths()["include"]]
@@ -149,6 +159,9 @@ def build_generation():
               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + inc +
              ["-L" + LIB, "-lchimera_b200", "-L" + tlib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
               "-Wl,-rpath,$ORIGIN/lib"])
+        os.makedirs(OBJ, exist_ok=True)
+        with open(stamp, "w") as f:
+            f.write(str(torch.__version__))
     return mod
 
 
