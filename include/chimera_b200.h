@@ -448,14 +448,17 @@ chm_status chm_cache_read(const chm_kv_cache* cache, const int64_t* slots, int64
  * or a length past the table's end, makes the sequence's rows and lse NaN.
  * An element with infinite values of one sign among those attended to is that
  * infinity; with both signs, or a NaN, it is NaN.
- * Softmax statistics and sums are fp32; probabilities enter the value product
- * as two 16-bit terms (high and remainder); beside 8-bit caches q enters the
- * score product as fp16, brought into its range by a power of two per row
- * (exact but for elements below 2^-28 of the row's largest), and where 8-bit
- * values pass 2^110 in magnitude, probabilities below 2^-16 of the largest may
- * count as zero.  A sequence may be cut elsewhere in another batch or with a
- * wider table, which moves the rounding of its sums; the same call gives the
- * same bits every time.
+ * Softmax statistics and sums are fp32.  Probabilities enter the value product
+ * in 16-bit terms: three over bf16 caches, which hold all of fp32's 24 bits, two
+ * fp16 ones over the others (22 bits, and nothing where a probability, times its
+ * value's scale beside 8-bit caches, is below 2^-36 of the row's largest).
+ * Beside 8-bit caches q enters the score product as fp16, brought into its range
+ * by a power of two per row (exact but for elements below 2^-28 of the row's
+ * largest), and where 8-bit values pass 2^110 in magnitude, probabilities below
+ * 2^-16 of the largest may count as zero.  Over bf16 caches a sum of magnitudes
+ * past 2^119 may come out infinite.  A sequence may be cut elsewhere in another
+ * batch or with a wider table, which moves the rounding of its sums; the same
+ * call gives the same bits every time.
  * table_width * page_size is at most 2^30, batch 65,535, and the keys' and the
  * values' memory span at most 64 GB each.  Calls on one workspace must not
  * overlap.  The workspace of sizes that a call refuses is 0 bytes, the reason in

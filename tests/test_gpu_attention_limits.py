@@ -169,3 +169,30 @@ def test_queries_from_the_ends_of_bf16(held, up):
     assert bool(c.ks.isfinite().all() & (c.ks >= 2.0 ** -126).logical_or(c.ks == 0).all())
     got, lse = c.run(scale=0.004)
     assert torch.equal(got, want) and torch.equal(lse, wlse)
+
+
+@pytest.mark.parametrize("held,t", [("bf16", None), ("fp16", None), ("int8", "bf16")])
+def test_weights_keep_what_fp32_holds(held, t):
+    """Three tokens whose values cancel, for 256 weights w: 1 * 1 - w (c1 + c2) with c1 + c2 next to 1 / w, so that the
+    output shows a weight's own error.  The exponents' difference is below 0.87 and off by at most 9 roundings of it
+    (5.5 u of the weight), exp2 by 2^-22; three products of 3 terms are summed, each off by at most 2 u of the largest
+    (18 u): together below 2^-19 of sum p |v|."""
+    b = 256
+    c = Case(lens=[3] * b, q_heads=1, k_heads=1, dim=64, page=3, held=held, t=t)
+    x = torch.linspace(0.01, 0.99, b, device=DEV).to(c.t)
+    w = torch.exp(0.6 * (x.double() - 1))
+    k = torch.zeros(b, 3, 64, device=DEV)
+    v = torch.zeros(b, 3, 64, device=DEV)
+    k[:, 0, 0], k[:, 1, 0], k[:, 2, 0] = 1, x.float(), x.float()
+    v[:, 0] = 1
+    v[:, 1] = -(1 / w).to(c.t).float()[:, None]
+    v[:, 2] = -(1 / w + v[:, 1, 0]).to(c.t).float()[:, None]
+    slots = (c.tables[:, :1].long() * 3 + torch.arange(3, device=DEV)).flatten()
+    A.cache_write(k.view(-1, 1, 64), v.view(-1, 1, 64), slots, c.kp, c.vp, c.ks, c.vs)
+    c.q.zero_()
+    c.q[:, 0, 0] = 1
+    got, lse = c.run(scale=0.6)
+    kk, vv = (c.values(p, s)[c.tables[:, 0].long(), 0] for p, s in ((c.kp, c.ks), (c.vp, c.vs)))
+    p = torch.softmax(0.6 * kk[..., 0], -1)[..., None]
+    want = (p * vv).sum(1)
+    within(got[:, 0], want, 2.0 ** -19 * (p * vv.abs()).sum(1) + torch.finfo(c.t).eps / 2 * want.abs() + 2.0 ** -25)
