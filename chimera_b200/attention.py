@@ -24,7 +24,9 @@ TypeError or ValueError before anything is launched; so do tensors that
 require a gradient while gradients are recorded, and tensors with a
 forward-mode tangent.  Tensors that a call writes (outputs given to it, pages,
 scales) count as modified in place; one whose vectors share memory (an expanded
-one), or that starts where another one does, is refused.
+one), or that starts where another one does, is refused.  The calls are plain
+functions, not registered operators: torch.compile breaks its graph at them, and
+torch.export cannot hold them.
 """
 from __future__ import annotations
 
@@ -50,7 +52,8 @@ def rotary_frequencies(rot_dim, base=10000.0, *, kind="plain", factor=1.0, origi
     `rotary`, for contexts up to `factor` times longer than `original_len`:
     "plain" (unscaled), "linear" (all divided by the factor), "base" (a larger
     base) or "parts" (pairs that turn more than `fast` times over original_len
-    as they are, fewer than `slow` times divided, a ramp between)."""
+    as they are, fewer than `slow` times divided, between them a ramp that is
+    linear in the number of turns, not in the pair's index)."""
     if kind not in KINDS:
         raise ValueError(f"kind must be one of {sorted(KINDS)}")
     rot_dim = int(rot_dim)

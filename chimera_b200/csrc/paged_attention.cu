@@ -14,18 +14,19 @@
 // runs are its operand registers as they come; 8-bit codes become fp16 numbers in
 // registers.  (tcgen05 would take K and V from shared memory only: codes would go
 // there a second time, and values transposed.  At 8 cycles per product the tensor
-// cores are busy for 15 to 25% of the time as it is.)  Each warp copies its runs
+// cores are busy for 9 to 20% of the time as it is.)  Each warp copies its runs
 // into a ring of its own in shared memory ahead of their use.
 //
-// One B200, us per call: 64 sequences of up to 4,096 tokens (32 query heads on 8
-// key heads of 128, bf16) 99 for 546 MB, 5.5 TB/s; one sequence of 262,144 tokens
-// (28 on 4 of 128, int8) 62 for 277 MB, 4.4 TB/s; 128 documents of up to 2,000
-// tokens (20 on 4 of 64, e4m3) 37 for 72 MB.  A call that joins parts costs about 10
-// for no tokens at all: two launches, some 3 us from a block's start to its first
-// product, 1 to 2 at each segment's end.  Past that, 16-bit caches stream at 6.5 TB/s;
-// 8-bit ones are bound by the instructions of 10 to 12 warps per SM beside that (0.56
-// issued per cycle; more warps, fewer instructions or shorter chains of products
-// did not change the time).
+// One B200, us on the device: 64 sequences of up to 4,096 tokens (32 query heads on
+// 8 key heads of 128, bf16) 94 for 546 MB, 5.8 TB/s; one sequence of 262,144 tokens
+// (28 on 4 of 128, int8) 58 for 277 MB, 4.8 TB/s; 128 documents of up to 2,000
+// tokens (20 on 4 of 64, e4m3) 35 for 72 MB (as calls among others 99, 65 and 37).
+// A call that joins parts costs 6 for one sequence of no tokens and
+// 14 for 128 of them: two launches, some 3 us from a block's start to its first
+// product, 1 to 2 at each segment's end.  Beside that, 16-bit caches wait for memory;
+// 8-bit ones are bound by the instructions of 10 to 12 warps per SM (0.56 issued per
+// cycle; more warps, fewer instructions or shorter chains of products did not change
+// the time).
 #include <algorithm>
 #include <cmath>
 #include <cstdio>
@@ -1072,7 +1073,11 @@ struct Launch {
         // of 1 / 16 / 64 / 128 sequences (32 query heads on 8 of 128, bf16): 2 tiles 6.2 / 6.3 /
         // 14 / 20 us whole, 7.0 / 10.4 / 16 / 23 split; 4 tiles 7.7 / 8.1 / 19 / 31 and 7.1 / 10.3 /
         // 18 / 33; 8 tiles 11.0 / 11.2 / 32 / 52 and 7.6 / 12.4 / 31 / 52, of 32 and 48 sequences
-        // 13.6 and 17.4 whole, 16.5 and 21.8 split.
+        // 13.6 and 17.4 whole, 16.5 and 21.8 split.  So one sequence of 4 tiles loses 0.6 us by
+        // the rule and 64 lose 1; 16 and 128 gain 2.  Whole segments are one unit whatever their
+        // length, and a block takes a whole number of them: past a round of the resident blocks
+        // (444 segments, 55 sequences of 8 key heads) the time steps up, 48 sequences of 256 tokens
+        // 11.8 us, 56 of them 17.8.
         const int whole = ((int64_t)a.batch * y.segs >= 128 ? 8 : 4) * S::kTile;
         y.unit_tokens = a.capacity <= whole ? whole : S::kTile;
         y.joins = a.capacity > whole;
@@ -1166,7 +1171,7 @@ struct Launch {
 // Calls f on the Launch<> for a cache's type, dim and sharing.  More than 8
 // query heads per key head take two blocks of 8 at a time, so that up to 16
 // read the cache once: 32 sequences of 4,096 tokens, 2 key heads of 128, bf16, 16 /
-// 9 query heads each 35 / 34 us, by single blocks 38 / 37; 128 sequences of 128
+// 9 query heads each 36 / 34 us, by single blocks 38 / 37; 128 sequences of 128
 // tokens 13 against 17 (one of 8,192 tokens 14 against 12).  At dim 256 the
 // registers hold one block.
 template <int KIND, typename F>

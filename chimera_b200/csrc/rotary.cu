@@ -7,9 +7,10 @@
 // whole turns at far positions; what is left takes 32-bit sine and cosine.
 //
 // HBM bounds it: each vector is read and written once.  One B200: a 16,384-token
-// prompt (32 + 8 heads of 128, bf16) 58 us for 336 MB, 5.8 TB/s; the gradient of 6,141
-// tokens of 24 heads of 96 (64 of them turned, neighbours, fp16) 15 us for 57 MB: 1.7
-// rounds of 6,141 warps, whose first bytes and angles take some 4 us.
+// prompt (32 + 8 heads of 128, bf16) 55 us on the device and 59 as a call for 336 MB, 5.7
+// to 6.1 TB/s; the gradient of 6,141 tokens of 24 heads of 96 (64 of them turned,
+// neighbours, fp16) 13 to 15 us for 57 MB: 1.7 rounds of 6,141 warps, whose first bytes
+// and angles take some 4 us, and 6 of 8 lanes at work.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
