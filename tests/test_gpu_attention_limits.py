@@ -196,3 +196,30 @@ def test_weights_keep_what_fp32_holds(held, t):
     p = torch.softmax(0.6 * kk[..., 0], -1)[..., None]
     want = (p * vv).sum(1)
     within(got[:, 0], want, 2.0 ** -19 * (p * vv.abs()).sum(1) + torch.finfo(c.t).eps / 2 * want.abs() + 2.0 ** -25)
+
+
+@pytest.mark.parametrize("n", [90, 9000])
+def test_infinite_values_beside_infinite_and_nan_keys(n):
+    """A NaN key makes its rows NaN whatever the values; where all scores are -inf the row is zeros and -inf, the
+    values infinite or not; the other heads of the same call have their infinities."""
+    c = Case(lens=[n, 300, 300], q_heads=12, k_heads=2, dim=64, page=16, held="bf16", seed=n)
+    clean, clse = c.run()
+    c.vp[..., 5] = math.inf
+    c.vp[c.tables[2, :19].long(), 1, :, 6] = -math.inf
+    for j in range(300):
+        p, w = place(c, 1, j)
+        c.kp[p, 0, w] = 0
+        c.kp[p, 0, w, 0] = -math.inf
+    c.q[1, :, 0] = 1.0
+    c.q[0, 3, 9] = math.nan
+    got, lse = c.run()
+    assert bool(got[0, 3].isnan().all() & lse[0, 3].isnan())
+    assert bool((got[1, :6] == 0).all() & (lse[1, :6] == -math.inf).all())
+    rows = [(0, h) for h in range(12) if h != 3] + [(1, h) for h in range(6, 12)] + [(2, h) for h in range(12)]
+    for b, h in rows:
+        assert float(got[b, h, 5]) == math.inf
+        assert b != 2 or h < 6 or float(got[b, h, 6]) == -math.inf
+        rest = [d for d in range(64) if d != 5 and not (b == 2 and h > 5 and d == 6)]
+        assert bool(got[b, h, rest].isfinite().all()) and bool(lse[b, h].isfinite())
+        if b != 1:
+            assert torch.equal(got[b, h, rest], clean[b, h, rest]) and torch.equal(lse[b, h], clse[b, h])
